@@ -42,7 +42,7 @@ extern "C" {
 const char* kvt_last_error(void);
 /* sizeof() of the ABI structs as compiled, for binding self-checks:
  * which = 0 kvt_ipc_block, 1 kvt_worker_info, 2 kvt_task, 3 kvt_parse_opts,
- * 4 kvt_xform, 5 kvt_wire_layout, 6 kvt_run. */
+ * 4 kvt_xform, 5 kvt_wire_layout, 6 kvt_run, 7 kvt_kv_layout, 8 kvt_rotary_opts. */
 uint64_t kvt_abi_sizeof(int which);
 /* Number of usable gfx950 devices (0 when none / no driver). */
 int kvt_device_count(void);
@@ -849,6 +849,101 @@ typedef struct kvt_object_ring_counters {
   uint64_t entries_in_use;        /* keys in the index now                                       */
 } kvt_object_ring_counters;
 int kvt_object_ring_stats(kvt_object_ring* r, kvt_object_ring_counters* out);
+
+/* ------------------------- operators on the registered cache: what fills and reads its pages */
+
+/* No counterpart in the reference, whose engine brings these with it: the three operators an
+ * engine runs on the pages that the calls above move -- rotary positions, the append of a step's
+ * keys and values to the pages, and the attention of one new token over them. They take the
+ * cache as it is registered for the transfer (kvt_cache) and the layouts of its cache shapes, run
+ * on the caller's stream, allocate nothing, synchronise nothing and can be captured into a hipGraph.
+ * Device arrays (positions, slots, block tables, lengths) are read by the kernels alone; a value
+ * in them that names no row of the cache is skipped there as stated below, never followed. */
+
+enum { KVT_DTYPE_BF16 = 0, KVT_DTYPE_F16 = 1, KVT_DTYPE_F32 = 2, KVT_DTYPE_E4M3 = 3 };
+
+/* Where the row of (block, K or V, token of the block, KV head) lies in a layer's tensor: at
+ * block * block_stride + which * kv_stride + token * token_stride + head * head_stride bytes,
+ * head_dim elements of dtype (BF16, F16, or E4M3: the OCP type the converting pack writes).
+ * Accepted are head_dim a multiple of 16 up to 256, strides and layer pointers that are multiples
+ * of 16 bytes, ntpb up to 65536, n_blocks below 2^31, and strides that keep all rows apart. */
+typedef struct kvt_kv_layout {
+  uint32_t dtype;
+  uint32_t tensor;        /* which tensor of the layer (0 where a layer has one) */
+  uint32_t n_kv_heads;
+  uint32_t head_dim;
+  uint32_t ntpb;          /* tokens per block */
+  uint32_t reserved0;
+  uint64_t n_blocks;
+  uint64_t block_stride, kv_stride, token_stride, head_stride;
+} kvt_kv_layout;
+
+/* The layout of a dense cache of `cache_shape`: KVT_SHAPE_FLASH, _RAGGED_FLASH, _FLASHINFER
+ * (HND pages), _QWEN3_NEXT_FLASH and _QWEN3_NEXT_FLASHINFER (their attention pages; for pages that
+ * bundle several kernel blocks, n_blocks and ntpb count kernel blocks, see kvt_enlarge_block_ids).
+ * KVT_ERR_UNSUPPORTED for the shapes whose rows are not keys and values per head (MLA, KDA). */
+int kvt_kv_layout_of(int cache_shape, uint32_t dtype, uint64_t n_blocks, uint32_t ntpb,
+                     uint32_t n_kv_heads, uint32_t head_dim, kvt_kv_layout* out);
+
+/* Rotary positions. Pair i of a row turns by position * freq[i] radians: elements (i, i +
+ * rotary_dim / 2), or (2 i, 2 i + 1) where interleaved; elements from rotary_dim on stay as they
+ * are. (x0, x1) -> magnitude * (x0 cos - x1 sin, x0 sin + x1 cos), in 32 bits from an angle that
+ * is formed and reduced to a turn in 64, rounded once to the output's type.
+ * Frequencies: KVT_ROTARY_PLAIN base^(-2i / rotary_dim); _LINEAR that / factor; _BANDS: a pair
+ * that makes at least `high` turns over original_max_position keeps its frequency, one that makes
+ * at most `low` has it divided by factor, in between the two are mixed linearly in the turns;
+ * _RAMP (the "NTK by parts" of the YaRN paper): mixed linearly in the pair's number between the
+ * pairs that make `high` and `low` turns (rounded outwards), and magnitude 0.1 ln(factor) + 1
+ * (1 where factor <= 1). low / high = 0 stand for 1 and 4 (_BANDS), 1 and 32 (_RAMP);
+ * magnitude = 0 for the kind's own. */
+enum { KVT_ROTARY_PLAIN = 0, KVT_ROTARY_LINEAR = 1, KVT_ROTARY_BANDS = 2, KVT_ROTARY_RAMP = 3 };
+typedef struct kvt_rotary_opts {
+  uint32_t rotary_dim;    /* even, 2 ... 256 */
+  uint32_t scaling;       /* KVT_ROTARY_* */
+  double base, factor, original_max_position, low, high, magnitude;
+} kvt_rotary_opts;
+/* freq[0 .. rotary_dim / 2) and *magnitude of these options. Host only. */
+int kvt_rotary_frequencies(const kvt_rotary_opts* opts, double* freq, double* magnitude);
+/* A rotation: immutable, holds no device memory (its frequencies travel with every launch), may
+ * be used on any device and from any number of threads. */
+typedef struct kvt_rotary kvt_rotary;
+int kvt_rotary_create(uint32_t rotary_dim, int interleaved, const double* freq, double magnitude,
+                      kvt_rotary** out);
+void kvt_rotary_destroy(kvt_rotary* r);
+/* out[t, h, :] = x[t, h, :] rotated to positions[t], for n_tokens x n_heads rows of head_dim
+ * elements of dtype (BF16, F16 or F32; head_dim >= rotary_dim, up to 256 and of any size
+ * otherwise). Rows at token * token_stride + head * head_stride bytes, elements of a row next to
+ * each other. out == x with the same strides rotates in place; an output that otherwise shares
+ * bytes with x is refused, and so are output strides that let rows meet. positions: int64, on the
+ * device, may be negative. Pointers and strides that are multiples of 16 bytes, with head_dim and
+ * rotary_dim multiples of 16, take the vector path, anything aligned to the element a slower one. */
+int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void* x,
+                     uint64_t x_token_stride, uint64_t x_head_stride, void* out,
+                     uint64_t out_token_stride, uint64_t out_head_stride, const int64_t* positions,
+                     uint64_t n_tokens, uint32_t n_heads, uint32_t head_dim, void* stream);
+
+/* Appends a step's keys and values to layer `layer` of the cache and rotates its queries, in one
+ * launch: token t goes to row slots[t] = block * ntpb + token of the block (int64, on the device).
+ *   K row = round(rotated k[t, h] / k_scale), V row = round(v[t, h] / v_scale)
+ *   q_out[t, h] = rotated q[t, h]          (q = NULL, n_q_heads = 0: no queries)
+ * rotary = NULL: nothing is rotated (positions may be NULL) and q must be NULL. dtype (BF16 or
+ * F16) is that of k, v and q; the cache holds the same type, or E4M3, rounded once from 32 bits,
+ * to nearest even, saturating at +-448, NaN staying NaN, as the converting pack does (which has no
+ * scales: pages that it is to produce or meet take scales of 1). For a cache of 16 bits the
+ * scales must be 1. The reciprocals of the scales are multiplied with. q_out may be q itself (same
+ * strides); sharing bytes with q otherwise, or with k or v, is refused.
+ * slots[t] outside [0, n_blocks * ntpb) -- padding, -1 -- leaves the cache alone (the query row
+ * is rotated all the same); every other row of the cache keeps its bytes. Two tokens of one call
+ * with the same slot leave an unspecified mixture of their rows in it. Inputs may be slices of a
+ * wider tensor (strides as in kvt_rotary_apply). */
+int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* layout,
+                  const kvt_rotary* rotary, uint32_t dtype, const void* k, uint64_t k_token_stride,
+                  uint64_t k_head_stride, const void* v, uint64_t v_token_stride,
+                  uint64_t v_head_stride, const void* q, uint64_t q_token_stride,
+                  uint64_t q_head_stride, uint32_t n_q_heads, void* q_out,
+                  uint64_t q_out_token_stride, uint64_t q_out_head_stride,
+                  const int64_t* positions, const int64_t* slots, uint64_t n_tokens, float k_scale,
+                  float v_scale, void* stream);
 
 /* ------------------------------------------------------------- utilities */
 

@@ -122,6 +122,8 @@ uint64_t kvt_abi_sizeof(int which) {
     case 4: return sizeof(kvt_xform);
     case 5: return sizeof(kvt_wire_layout);
     case 6: return sizeof(kvt_run);
+    case 7: return sizeof(kvt_kv_layout);
+    case 8: return sizeof(kvt_rotary_opts);
     default: return 0;
   }
 }

@@ -32,6 +32,17 @@ class Xform(C.Structure):
     _fields_ = [("kind", _u32), ("heads", _u32), ("ntpb", _u32), ("row_bytes", _u32)]
 
 
+class KvLayoutStruct(C.Structure):
+    _fields_ = [("dtype", _u32), ("tensor", _u32), ("n_kv_heads", _u32), ("head_dim", _u32),
+                ("ntpb", _u32), ("reserved0", _u32), ("n_blocks", _u64), ("block_stride", _u64),
+                ("kv_stride", _u64), ("token_stride", _u64), ("head_stride", _u64)]
+
+
+class RotaryOpts(C.Structure):
+    _fields_ = [("rotary_dim", _u32), ("scaling", _u32)] + [
+        (n, C.c_double) for n in ("base", "factor", "original_max_position", "low", "high", "magnitude")]
+
+
 # name -> (restype, argtypes); this table is also what tests/test_abi.py checks
 # against the declarations in include/kvt_hip.h.
 SIGNATURES = {
@@ -156,6 +167,13 @@ SIGNATURES = {
     "kvt_stager_wait": (_int, [_vp, _u32]),
     "kvt_measure_pcie": (_int, [_int, _int, _u64, _u32, _P(C.c_double)]),
     "kvt_measure_pcie_both_ways": (_int, [_int, _u64, _u32, _P(C.c_double), _P(C.c_double)]),
+    "kvt_kv_layout_of": (_int, [_int, _u32, _u64, _u32, _u32, _u32, _P(KvLayoutStruct)]),
+    "kvt_rotary_frequencies": (_int, [_P(RotaryOpts), _P(C.c_double), _P(C.c_double)]),
+    "kvt_rotary_create": (_int, [_u32, _int, _P(C.c_double), C.c_double, _P(_vp)]),
+    "kvt_rotary_destroy": (None, [_vp]),
+    "kvt_rotary_apply": (_int, [_vp, _int, _u32, _vp, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u32, _u32, _vp]),
+    "kvt_kv_append": (_int, [_vp, _u32, _vp, _vp, _u32] + [_vp, _u64, _u64] * 3 + [_u32, _vp, _u64, _u64, _vp, _vp,
+                             _u64, C.c_float, C.c_float, _vp]),
     "kvt_copy_linear": (_int, [_vp, _vp, _u64, _vp]),
     "kvt_copy_runtime_d2d": (_int, [_vp, _vp, _u64, _vp]),
     "kvt_event_create": (_int, [_P(_vp)]),

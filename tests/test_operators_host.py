@@ -1,0 +1,183 @@
+"""The host side of the operators on the paged cache: layouts of the cache shapes, frequencies of
+rotary positions, and the calls that are refused before anything reaches a device. CPU only."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+import kvt_amd
+import operator_cases as oc
+from kvt_amd import binding, ctypes_defs
+from kvt_amd.ctypes_defs import ERR_INVALID, ERR_UNSUPPORTED
+
+
+def _refused(code, fn, *args, **kw):
+    with pytest.raises(kvt_amd.KvtError) as e:
+        fn(*args, **kw)
+    assert e.value.code == code, e.value
+    return str(e.value)
+
+
+def test_struct_sizes_match():
+    assert kvt_amd.lib().kvt_abi_sizeof(7) == C.sizeof(binding.KvLayoutStruct)
+    assert kvt_amd.lib().kvt_abi_sizeof(8) == C.sizeof(binding.RotaryOpts)
+
+
+@pytest.mark.parametrize("dtype,size", [("bf16", 2), ("f16", 2), ("e4m3", 1)])
+@pytest.mark.parametrize("layout", sorted(oc.SHAPES))
+@pytest.mark.parametrize("n,block,heads,dim", [(7, 16, 8, 128), (3, 1, 1, 16), (5, 24, 3, 80), (1, 544, 2, 256)])
+def test_layout_of_a_cache_shape_is_where_numpy_finds_the_rows(layout, dtype, size, n, block, heads, dim):
+    a = np.arange(2 * n * block * heads * dim, dtype=np.int64).reshape(oc.cache_shape(layout, n, block, heads, dim))
+    views = oc.kv_views(layout, a)
+    s = kvt_amd.KvLayout(oc.SHAPES[layout], dtype, n, block, heads, dim).struct
+    for which in (0, 1):
+        for b, t, h in ((0, 0, 0), (n - 1, block - 1, heads - 1), (n // 2, block // 2, heads // 2)):
+            at = b * s.block_stride + which * s.kv_stride + t * s.token_stride + h * s.head_stride
+            assert at == int(views[which][b, t, h, 0]) * size
+
+
+@pytest.mark.parametrize("shape", [ctypes_defs.SHAPE_DPSK_V32_SPARSE_MLA, ctypes_defs.SHAPE_KIMI_K3_MLA,
+                                   ctypes_defs.SHAPE_TURBOQUANT, 0, 99])
+def test_layouts_without_keys_and_values_per_head_are_refused(shape):
+    _refused(ERR_UNSUPPORTED, kvt_amd.KvLayout, shape, "bf16", 8, 16, 1, 64)
+
+
+@pytest.mark.parametrize("n,block,heads,dim", [(0, 16, 8, 128), (8, 0, 8, 128), (8, 16, 0, 128), (1 << 31, 16, 8, 128),
+                                               (8, 65537, 8, 128), (8, 16, 65537, 128)])
+def test_layout_sizes_out_of_range_are_refused(n, block, heads, dim):
+    _refused(ERR_INVALID, kvt_amd.KvLayout, ctypes_defs.SHAPE_FLASH, "bf16", n, block, heads, dim)
+
+
+@pytest.mark.parametrize("dim", [0, 8, 24, 100, 272])
+def test_head_sizes_that_are_no_multiple_of_16_up_to_256_are_refused(dim):
+    for shape in (ctypes_defs.SHAPE_FLASH, ctypes_defs.SHAPE_FLASHINFER):
+        with pytest.raises(kvt_amd.KvtError) as e:
+            kvt_amd.KvLayout(shape, "bf16", 8, 16, 8, dim)
+        assert e.value.code in (ERR_INVALID, ERR_UNSUPPORTED)
+
+
+def test_frequencies_are_the_formulas():
+    d, base, f, length = 64, 10000.0, 8.0, 4096
+    plain = [base ** (-2 * i / d) for i in range(d // 2)]
+    got, m = kvt_amd.rotary_frequencies(d, base)
+    assert np.allclose(got, plain, rtol=1e-14, atol=0) and m == 1.0
+    got, m = kvt_amd.rotary_frequencies(d, base, "linear", f)
+    assert np.allclose(got, [w / f for w in plain], rtol=1e-14, atol=0) and m == 1.0
+    got, m = kvt_amd.rotary_frequencies(d, base, "bands", f, length)
+    for w, g in zip(plain, got):
+        turns = length * w / (2 * math.pi)
+        mix = 0 if turns >= 4 else 1 if turns <= 1 else (4 - turns) / 3
+        assert math.isclose(g, w * (1 - mix) + w / f * mix, rel_tol=1e-13)
+    assert m == 1.0 and got[0] == plain[0] and math.isclose(got[-1], plain[-1] / f, rel_tol=1e-14)
+    got, m = kvt_amd.rotary_frequencies(d, base, "ramp", f, length)
+    pair = lambda turns: d * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+    lo, hi = math.floor(pair(32)), math.ceil(pair(1))
+    for i, (w, g) in enumerate(zip(plain, got)):
+        mix = min(1, max(0, (i - lo) / (hi - lo)))
+        assert math.isclose(g, w * (1 - mix) + w / f * mix, rel_tol=1e-13)
+    assert math.isclose(m, 0.1 * math.log(f) + 1)
+    assert kvt_amd.rotary_frequencies(d, base, "ramp", f, length, magnitude=0.5)[1] == 0.5
+    assert kvt_amd.rotary_frequencies(d, base, "ramp", 0.5, length)[1] == 1.0
+
+
+@pytest.mark.parametrize("dim,kw", [
+    (0, {}), (3, {}), (258, {}), (64, dict(base=1.0)), (64, dict(base=math.nan)), (64, dict(scaling="linear", factor=0.0)),
+    (64, dict(scaling="bands", factor=8.0)), (64, dict(scaling="ramp", factor=8.0, original_max_position=-1.0)),
+    (64, dict(scaling="bands", factor=8.0, original_max_position=4096, low=4.0, high=4.0)),
+    (64, dict(scaling="linear", factor=math.inf)), (64, dict(magnitude=-1.0))])
+def test_frequencies_out_of_range_are_refused(dim, kw):
+    _refused(ERR_INVALID, kvt_amd.rotary_frequencies, dim, **kw)
+
+
+def test_rotations_out_of_range_are_refused():
+    for bad in ([math.nan] + [1.0] * 31, [math.inf] + [1.0] * 31):
+        _refused(ERR_INVALID, kvt_amd.Rotary, 64, frequencies=bad)
+    _refused(ERR_INVALID, kvt_amd.Rotary, 64, frequencies=[1.0] * 32, magnitude=math.inf)
+    with pytest.raises(ValueError):
+        kvt_amd.Rotary(64, frequencies=[1.0] * 31)
+    lib = kvt_amd.lib()
+    assert lib.kvt_rotary_create(64, 0, None, 1.0, None) == ERR_INVALID
+    lib.kvt_rotary_destroy(None)
+
+
+# The calls below are refused on the host: the pointers are never followed.
+P, POS = 1 << 20, 1 << 30
+
+
+def _apply(r, **kw):
+    a = dict(device=0, dtype=0, x=P, x_tok=1024, x_head=128, out=2 * P, out_tok=1024, out_head=128, positions=POS,
+             n=64, heads=8, dim=64)
+    a.update(kw)
+    return kvt_amd.lib().kvt_rotary_apply(r.h if r else None, *a.values(), None)
+
+
+def test_rotary_apply_refuses_on_the_host():
+    r = kvt_amd.Rotary(64)
+    assert _apply(None) == ERR_INVALID
+    assert _apply(r, dtype=3) == ERR_UNSUPPORTED and _apply(r, dtype=9) == ERR_UNSUPPORTED
+    assert _apply(r, dim=62) == ERR_INVALID and _apply(r, dim=257) == ERR_INVALID
+    assert _apply(r, x=None) == ERR_INVALID and _apply(r, out=None) == ERR_INVALID
+    assert _apply(r, positions=None) == ERR_INVALID and _apply(r, positions=POS + 4) == ERR_INVALID
+    assert _apply(r, x=P + 1) == ERR_INVALID and _apply(r, out_tok=1025) == ERR_INVALID
+    assert _apply(r, out_head=126) == ERR_INVALID                    # rows of the output meet
+    assert _apply(r, out_tok=512) == ERR_INVALID
+    assert _apply(r, out=P + 2) == ERR_INVALID                       # shares bytes with x
+    assert _apply(r, out=P + 1024) == ERR_INVALID
+    assert _apply(r, out=P, out_tok=2048) == ERR_INVALID             # in place with other strides
+    assert _apply(r, n=1 << 62, x_tok=0, out_tok=1 << 20) == ERR_INVALID
+    last = kvt_amd.lib().kvt_last_error()
+    assert b"kvt_rotary_apply" in last
+
+
+@pytest.mark.skipif(kvt_amd.device_count() > 0, reason="this check is for machines without a GPU")
+def test_calls_that_are_right_need_a_device():
+    r = kvt_amd.Rotary(64)
+    assert _apply(r) == ctypes_defs.ERR_NO_DEVICE
+    assert _apply(r, out=P) == ctypes_defs.ERR_NO_DEVICE             # in place
+    # two halves of one wider tensor: interleaved, no byte shared
+    assert _apply(r, x_tok=2048, out=P + 1024, out_tok=2048) == ctypes_defs.ERR_NO_DEVICE
+    assert _apply(r, x=P + 1024, x_tok=2048, out=P, out_tok=2048) == ctypes_defs.ERR_NO_DEVICE
+
+
+def _append(layout, rotary, **kw):
+    a = dict(dtype=0, k=P, k_tok=4096, k_head=256, v=P + 2048, v_tok=4096, v_head=256, q=4 * P, q_tok=8192, q_head=256,
+             q_heads=32, q_out=8 * P, qo_tok=8192, qo_head=256, positions=POS, slots=2 * POS, n=8, k_scale=1.0,
+             v_scale=1.0)
+    a.update(kw)
+    return kvt_amd.lib().kvt_kv_append(None, 0, layout.ref if layout else None, rotary.h if rotary else None,
+                                       *a.values(), None)
+
+
+def test_append_refuses_on_the_host():
+    lay = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128)
+    lay8 = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "e4m3", 64, 16, 8, 128)
+    r = kvt_amd.Rotary(128)
+    said = lambda: kvt_amd.lib().kvt_last_error()  # noqa: E731
+    assert _append(lay, r) == ERR_INVALID and b"null cache" in said()    # everything else is right
+    assert _append(lay, None, q=None, q_heads=0, positions=None) == ERR_INVALID and b"null cache" in said()
+    assert _append(lay8, r, k_scale=0.5) == ERR_INVALID and b"null cache" in said()
+    assert _append(None, r) == ERR_INVALID and b"null layout" in said()
+    assert _append(lay, r, dtype=2) == ERR_UNSUPPORTED and _append(lay, r, dtype=1) == ERR_UNSUPPORTED
+    assert _append(lay, r, k_scale=2.0) == ERR_INVALID and b"scales" in said()
+    for bad in (0.0, -1.0, math.nan, math.inf, 1e-39):
+        assert _append(lay8, r, v_scale=bad) == ERR_INVALID and b"scales" in said()
+    assert _append(lay, None) == ERR_INVALID and b"rotation" in said()
+    assert _append(lay, kvt_amd.Rotary(256)) == ERR_INVALID and b"longer" in said()
+    assert _append(lay, r, slots=None) == ERR_INVALID and b"slots" in said()
+    assert _append(lay, r, positions=POS + 1) == ERR_INVALID and b"positions" in said()
+    assert _append(lay, r, k=None) == ERR_INVALID and _append(lay, r, q_out=None) == ERR_INVALID
+    assert _append(lay, r, q_out=P) == ERR_INVALID and b"shares bytes" in said()
+    assert _append(lay, r, q_out=4 * P, qo_tok=16384) == ERR_INVALID and b"shares bytes" in said()
+    # q rotated in place inside the fused tensor that holds k and v as well
+    fused = dict(q=P, q_tok=12288, q_out=P, qo_tok=12288, k=P + 8192, k_tok=12288, v=P + 10240, v_tok=12288)
+    assert _append(lay, r, **fused) == ERR_INVALID and b"null cache" in said()
+    assert _append(lay, r, **dict(fused, k=P + 8000)) == ERR_INVALID and b"shares bytes with k" in said()
+
+
+@pytest.mark.parametrize("strides", [(0, 1 << 16, 256, 4096), (65536, 256, 256, 4096), (65536, 1 << 22, 255, 4096),
+                                     (65536, 1 << 22, 4096, 128), (1 << 62, 1 << 61, 256, 4096)])
+def test_layouts_whose_rows_meet_are_refused(strides):
+    lay = kvt_amd.KvLayout(None, "bf16", 64, 16, 8, 128, strides=strides)
+    assert _append(lay, kvt_amd.Rotary(128)) == ERR_INVALID
+    assert b"null cache" not in kvt_amd.lib().kvt_last_error()
