@@ -945,6 +945,51 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
                   const int64_t* positions, const int64_t* slots, uint64_t n_tokens, float k_scale,
                   float v_scale, void* stream);
 
+/* Attention of one new token per sequence over its pages: for sequence b, query head h and the KV
+ * head g it shares with n_q_heads / n_kv_heads - 1 others,
+ *   s_t = softmax_scale k_scale q[b, h] . K[t, g]      (logit_cap tanh(s_t / logit_cap) where set)
+ *   out[b, h] = v_scale sum_t p_t V[t, g] / sum_t p_t, p_t = exp(s_t - max s)
+ *   lse[b, h] = ln sum_t exp(s_t)                      (float32, [n_seqs, n_q_heads]; NULL: not wanted)
+ * over the tokens t the sequence sees: its first seq_lens[b] tokens (the new one's row appended
+ * already), with a window the last `window` of them. Token t lies in block block_tables[b][t / ntpb].
+ * Not seen either: tokens behind the table's table_blocks columns, and those of a block id outside
+ * [0, n_blocks). A sequence that sees no token (a padding row: length 0 or negative) gets zeros and
+ * an lse of minus infinity. Rows of the cache that are not seen may hold anything, NaN included.
+ * Scores, weights, sums and the maximum are held in 32 bits, the weights take part in the product
+ * with V as two 16-bit values each; every output is rounded once. Results do not depend on the
+ * order in which workgroups run.
+ *
+ * An operator holds the layout, the heads and workspaces for sums of sequences that are split over
+ * several workgroups. It is meant to be kept: one serves all layers of a model and any number of
+ * caches of its layout on its device.
+ *   dtype           of q and out: BF16 or F16; the cache holds the same or E4M3
+ *   softmax_scale   0 = 1 / sqrt(head_dim)
+ *   logit_cap       0 = none;  window: 0 = none
+ *   max_seqs        most sequences of one call, up to 65535
+ *   n_workspaces    how many streams and captured graphs the operator serves during its life: each
+ *                   stream that launches it eagerly and each stream capture (per stream in it) takes
+ *                   one and keeps it, so that no two launches that may run at the same time share
+ *                   one; a call that finds none left is refused (KVT_ERR_INVALID). A graph must not
+ *                   run at the same time as a second instantiation of itself.
+ * Calls may come from several threads. Created and destroyed outside of stream captures; destroying
+ * it waits for the device. */
+typedef struct kvt_decode kvt_decode;
+int kvt_decode_create(int device, const kvt_kv_layout* layout, uint32_t dtype, uint32_t n_q_heads,
+                      float softmax_scale, float logit_cap, uint32_t window, uint32_t max_seqs,
+                      uint32_t n_workspaces, kvt_decode** out);
+void kvt_decode_destroy(kvt_decode* d);
+/* Gives back what `stream` holds: its eager workspace and those of the captures made on it. Call
+ * it when the stream's launches have run and its graphs are gone (before the stream is destroyed). */
+int kvt_decode_release(kvt_decode* d, void* stream);
+/* q, out: rows as in kvt_rotary_apply (out may not share bytes with q). block_tables: int32, row b
+ * at b * table_stride entries; seq_lens: int32. max_len: the longest length of the batch as far as
+ * the host knows it (0: the whole table); it decides how far sequences are split, never the result. */
+int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, const void* q,
+                         uint64_t q_token_stride, uint64_t q_head_stride, const int32_t* block_tables,
+                         uint64_t table_stride, uint32_t table_blocks, const int32_t* seq_lens,
+                         uint32_t n_seqs, uint64_t max_len, float k_scale, float v_scale, void* out,
+                         uint64_t out_token_stride, uint64_t out_head_stride, float* lse, void* stream);
+
 /* ------------------------------------------------------------- utilities */
 
 /* Plain device-to-device copy kernel with the same vector width and launch

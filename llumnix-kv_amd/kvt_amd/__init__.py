@@ -12,7 +12,7 @@ from .binding import (KvtError, LIB_PATH, BlockLists, RunLists, Cache, Parser, P
                       get_copy_cu_usage, ObjectRing, PlanSlot, SlotLayout, copy_ticket_stats)
 from .ctypes_defs import (SHAPE_FLASH, SHAPE_FLASHINFER, SHAPE_QWEN3_NEXT_FLASH,
                           SHAPE_QWEN3_NEXT_FLASHINFER, SHAPE_RAGGED_FLASH)
-from .operators import KvLayout, Rotary, kv_append, rotary_frequencies
+from .operators import DecodeAttention, KvLayout, Rotary, kv_append, rotary_frequencies
 from . import ctypes_defs
 
 __all__ = ["KvtError", "LIB_PATH", "BlockLists", "Cache", "Parser", "Plan", "Session", "Stager",
@@ -20,6 +20,6 @@ __all__ = ["KvtError", "LIB_PATH", "BlockLists", "Cache", "Parser", "Plan", "Ses
            "validate_bounds", "ctypes_defs", "WireLayout", "WIRE_TCP", "WIRE_RDMA_STAGED",
            "block_object_lists", "RunLists", "wire_layout_of", "wire_parse_frame", "wire_write_frame",
            "set_copy_cu_usage", "get_copy_cu_usage", "ObjectRing", "PlanSlot", "SlotLayout",
-           "copy_ticket_stats", "KvLayout", "Rotary", "kv_append", "rotary_frequencies",
+           "copy_ticket_stats", "DecodeAttention", "KvLayout", "Rotary", "kv_append", "rotary_frequencies",
            "SHAPE_FLASH", "SHAPE_FLASHINFER", "SHAPE_QWEN3_NEXT_FLASH",
            "SHAPE_QWEN3_NEXT_FLASHINFER", "SHAPE_RAGGED_FLASH"]

@@ -172,8 +172,14 @@ SIGNATURES = {
     "kvt_rotary_create": (_int, [_u32, _int, _P(C.c_double), C.c_double, _P(_vp)]),
     "kvt_rotary_destroy": (None, [_vp]),
     "kvt_rotary_apply": (_int, [_vp, _int, _u32, _vp, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u32, _u32, _vp]),
-    "kvt_kv_append": (_int, [_vp, _u32, _vp, _vp, _u32] + [_vp, _u64, _u64] * 3 + [_u32, _vp, _u64, _u64, _vp, _vp,
+    "kvt_kv_append": (_int, [_vp, _u32, _P(KvLayoutStruct), _vp, _u32] + [_vp, _u64, _u64] * 3 + [_u32, _vp, _u64, _u64, _vp, _vp,
                              _u64, C.c_float, C.c_float, _vp]),
+    "kvt_decode_create": (_int, [_int, _P(KvLayoutStruct), _u32, _u32, C.c_float, C.c_float, _u32, _u32, _u32,
+                                 _P(_vp)]),
+    "kvt_decode_destroy": (None, [_vp]),
+    "kvt_decode_release": (_int, [_vp, _vp]),
+    "kvt_decode_attention": (_int, [_vp, _vp, _u32, _vp, _u64, _u64, _vp, _u64, _u32, _vp, _u32, _u64, C.c_float,
+                                    C.c_float, _vp, _u64, _u64, _vp, _vp]),
     "kvt_copy_linear": (_int, [_vp, _vp, _u64, _vp]),
     "kvt_copy_runtime_d2d": (_int, [_vp, _vp, _u64, _vp]),
     "kvt_event_create": (_int, [_P(_vp)]),

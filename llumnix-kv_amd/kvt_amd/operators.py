@@ -38,7 +38,7 @@ def _rows(tensor, name, n_tokens, n_heads, dim, code):
 
 
 def _index(tensor, name, shape, dtype):
-    """Pointer of a contiguous integer tensor."""
+    """Pointer of a contiguous tensor of one type."""
     if tuple(tensor.shape) != shape or str(tensor.dtype) != dtype or not tensor.is_contiguous():
         raise ValueError("%s: expected a contiguous %s tensor of shape %s" % (name, dtype, shape))
     return tensor.data_ptr()
@@ -125,3 +125,41 @@ def kv_append(cache, layer, layout, k, v, slots, rotary=None, positions=None, q=
                               *_rows(v, "v", n, layout.n_kv_heads, dim, code), *q_args, q_heads, *out_args,
                               None if positions is None else _index(positions, "positions", (n,), "torch.int64"),
                               _index(slots, "slots", (n,), "torch.int64"), n, k_scale, v_scale, stream))
+
+
+class DecodeAttention:
+    """Attention of one new token per sequence over the paged cache (kvt_decode). One object serves
+    all layers; every stream that launches it and every stream capture takes one of `workspaces`."""
+
+    def __init__(self, device, layout, dtype, n_q_heads, max_seqs, softmax_scale=None, logit_cap=0.0, window=0,
+                 workspaces=4):
+        self.h = C.c_void_p()
+        self.layout, self.n_q_heads, self.code = layout, n_q_heads, DTYPES[dtype]
+        check(lib().kvt_decode_create(device, layout.ref, self.code, n_q_heads, softmax_scale or 0.0, logit_cap,
+                                      window, max_seqs, workspaces, C.byref(self.h)))
+
+    def run(self, cache, layer, q, block_tables, seq_lens, out, lse=None, max_len=0, k_scale=1.0, v_scale=1.0,
+            stream=None):
+        """q, out: [seqs, n_q_heads, head_dim]; block_tables: int32 [seqs, blocks]; seq_lens: int32 [seqs];
+        lse: float32 [seqs, n_q_heads] or None. max_len: the longest length if known. -> out"""
+        n, dim = q.shape[0], self.layout.head_dim
+        if (block_tables.dim() != 2 or block_tables.shape[0] != n or str(block_tables.dtype) != "torch.int32"
+                or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)):
+            raise ValueError("block_tables: expected int32 [%d, blocks] with contiguous rows" % n)
+        check(lib().kvt_decode_attention(
+            self.h, cache.h, layer, *_rows(q, "q", n, self.n_q_heads, dim, self.code), block_tables.data_ptr(),
+            block_tables.stride(0), block_tables.shape[1], _index(seq_lens, "seq_lens", (n,), "torch.int32"), n,
+            max_len, k_scale, v_scale, *_rows(out, "out", n, self.n_q_heads, dim, self.code),
+            None if lse is None else _index(lse, "lse", (n, self.n_q_heads), "torch.float32"), stream))
+        return out
+
+    def release(self, stream=None):
+        """Gives back the workspaces that `stream` and the captures made on it hold."""
+        check(lib().kvt_decode_release(self.h, stream))
+
+    def close(self):
+        if self.h:
+            lib().kvt_decode_destroy(self.h)
+            self.h = C.c_void_p()
+
+    __del__ = _quiet_close

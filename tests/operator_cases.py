@@ -66,18 +66,21 @@ def rotation_tolerance(exact, scale, kind):
 def decode_exact(q, keys, values, tables, lens, block, scale, window=0, cap=0.0, k_scale=1.0, v_scale=1.0):
     """Attention of one token per sequence in 64 bits: q [seqs, heads, dim], keys / values
     [n_blocks, block, kv_heads, dim] as float64; a page outside the cache is not seen.
-    -> (out, lse, sum of p |v|: what weights rounded on the way are measured by)"""
+    -> (out, lse, measure), measure = what decode_tolerance() goes by, per (sequence, head): the
+    sum of p |v| for every dim, the largest sum of |q k| of a score, tokens seen, the largest |v|."""
     n, heads, dim = q.shape
     n_blocks, _, kv_heads, _ = keys.shape
     group = heads // kv_heads
-    out, lse, mass = np.zeros((n, heads, dim)), np.full((n, heads), -np.inf), np.zeros((n, heads, dim))
+    out, lse = np.zeros((n, heads, dim)), np.full((n, heads), -np.inf)
+    mass, size, count, most = np.zeros((n, heads, dim)), np.zeros((n, heads)), np.zeros((n, heads)), np.zeros((n, heads))
     for b in range(n):
         length = max(0, min(int(lens[b]), tables.shape[1] * block))
         t = np.arange(max(0, length - window) if window else 0, length)
         if t.size == 0:
             continue
         page = tables[b][t // block].astype(np.int64)
-        t, page = t[(page >= 0) & (page < n_blocks)], page[(page >= 0) & (page < n_blocks)]
+        held = (page >= 0) & (page < n_blocks)
+        t, page = t[held], page[held]
         if t.size == 0:
             continue
         k, v = keys[page, t % block] * k_scale, values[page, t % block] * v_scale
@@ -86,10 +89,30 @@ def decode_exact(q, keys, values, tables, lens, block, scale, window=0, cap=0.0,
             if cap:
                 z = cap * np.tanh(z / cap)
             top = z.max()
-            with np.errstate(invalid="ignore"):
-                p = np.exp(z - top)
+            p = np.exp(z - top)
             lse[b, h] = top + np.log(p.sum())
             p = p / p.sum()
-            out[b, h] = p @ v[:, h // group]
-            mass[b, h] = p @ np.abs(v[:, h // group])
-    return out, lse, mass
+            out[b, h], mass[b, h] = p @ v[:, h // group], p @ np.abs(v[:, h // group])
+            size[b, h] = abs(scale) * (np.abs(k[:, h // group]) @ np.abs(q[b, h])).max()
+            count[b, h], most[b, h] = t.size, np.abs(v[:, h // group]).max()
+    return out, lse, (mass, size, count, most)
+
+
+def decode_tolerance(out, lse, measure, kind):
+    """(of out, of lse). In 32 bits a score is off by (dim + 8) 2^-24 of the sum of its |q k|: dim
+    additions, the scale, the change of base and the difference to the maximum (the products of two
+    16-bit values are exact); the weights of a softmax by twice that, relative, and 4 roundings of
+    the exponential. Sums over n tokens: n roundings of 2^-24 of the sum of p |v|. A weight in two
+    16-bit values, cut off (a step, 2^-7 for bf16 and 2^-10 for f16) and the rest rounded (half a
+    step): 2^-15 or 2^-21 of it; the rest is at least the smallest positive number, for f16 2^-24 of
+    every |v|, and rounded by half of that. Joining parts and dividing: 8 more. Then the output's own rounding."""
+    mass, size, count, most = measure
+    dim = out.shape[-1]
+    score = (dim + 8) * 2.0 ** -24 * size
+    split = 2.0 ** -15 if kind == "bf16" else 2.0 ** -21
+    rel = 2 * score + (12 + count) * 2.0 ** -24 + split
+    tol = rel[..., None] * mass + (0 if kind == "bf16" else 1.5 * 2.0 ** -24 * (count * most)[..., None])
+    half, floor = HALF_STEP[kind]
+    seen = np.isfinite(lse)
+    return (half * (np.abs(out) + tol) + floor + tol,
+            score + (16 + count + 2 * np.where(seen, np.abs(lse), 0) + 2 * size) * 2.0 ** -24)
