@@ -40,7 +40,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int kThreads = 256, kWaves = 4;
 constexpr uint32_t kTile = 32;                   // tokens a wavefront takes at a time
 constexpr uint32_t kStep = kTile * kWaves;       // ... and a workgroup
-constexpr uint32_t kMaxSplits = 256;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.69314718055994531f;
 
 struct DecodeParams {
@@ -54,11 +53,12 @@ struct DecodeParams {
   uint8_t* out;
   int64_t out_token, out_head;
   float* lse;
-  float* part_o;       // [seq][head][split][head_dim]: sums not yet divided
-  float2* part_ml;     // [seq][head][split]: maximum (times log2 e), sum
-  uint32_t* counters;  // [seq][group of heads]: workgroups that have left their part
-  uint64_t block_magic, visible_max;
-  uint32_t ntpb, n_blocks, n_heads, group, head_tiles, head_dim, window, chunk, splits;
+  float* part_o;       // [workgroup][first, last][head][head_dim]: sums not yet divided
+  float2* part_ml;     // [workgroup][first, last][head]: maximum (times log2 e), sum
+  uint32_t* counters;  // [workgroup]: parts of the row that starts in it that have been left
+  uint64_t block_magic;
+  uint32_t visible_max, ntpb, n_blocks, n_seqs, n_heads, head_dim, window;
+  uint32_t group, spread, head_rows, rows, teams, slot_heads;
   float scale_log2, cap, cap_in, v_scale;
   bool q_vec, out_vec;
 };
@@ -95,6 +95,40 @@ struct F16 {
   static constexpr float kLeast = 0x1p-24f;
 };
 
+// N pieces of 16 bytes from LDS, once all but the newest `NEWER` vector memory operations are done:
+// what loads that go to LDS have written is not there before, and the compiler, which does not tell
+// their targets apart, would wait for every load there is.
+template <int N, int NEWER>
+__device__ __forceinline__ void read_k(const uint32_t* at, int offset, u32x4* r) {
+  if constexpr (N == 1) {
+    if (offset == 0)
+      asm volatile("s_waitcnt vmcnt(%2)\n\tds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(r[0]) : "v"(at[0]), "n"(NEWER) : "memory");
+    else
+      asm volatile("ds_read_b128 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=&v"(r[0]) : "v"(at[0] + offset) : "memory");
+  } else if constexpr (N == 2) {
+    if (offset == 0)
+      asm volatile("s_waitcnt vmcnt(%4)\n\tds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(r[0]), "=&v"(r[1]) : "v"(at[0]), "v"(at[1]), "n"(NEWER) : "memory");
+    else
+      asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                   : "=&v"(r[0]), "=&v"(r[1]) : "v"(at[0] + offset), "v"(at[1] + offset) : "memory");
+  } else {
+#pragma unroll
+    for (int n = 0; n < N; n += 4) {
+      if (offset == 0 && n == 0)
+        asm volatile("s_waitcnt vmcnt(%8)\n\tds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\t"
+                     "ds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+                     : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(NEWER) : "memory");
+      else
+        asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\t"
+                     "ds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(r[n]), "=&v"(r[n + 1]), "=&v"(r[n + 2]), "=&v"(r[n + 3])
+                     : "v"(at[n] + offset), "v"(at[n + 1] + offset), "v"(at[n + 2] + offset), "v"(at[n + 3] + offset) : "memory");
+    }
+  }
+}
+
 // The maximum / sum over the four lanes that hold one head's tokens (lane, +16, +32, +48).
 __device__ __forceinline__ float over_tokens_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16));
@@ -103,6 +137,45 @@ __device__ __forceinline__ float over_tokens_max(float v) {
 __device__ __forceinline__ float over_tokens_sum(float v) {
   v += __shfl_xor(v, 16);
   return v + __shfl_xor(v, 32);
+}
+
+// Cache policies of the buffer instructions: bit 1 = non-temporal (rows of the cache are read
+// once), bit 4 = sc1, the scope of the device.
+constexpr int kStreamed = 2, kShared = 16;
+template <class V>
+__device__ __forceinline__ V streamed(const uint8_t* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+}
+
+// Parts of split sequences pass from one workgroup to another, on whatever XCD: written through
+// to, and read from, where all XCDs see them (sc1: the scope of the device).
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t rsrc_of(void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7FFFFFFF, 0x00020000);
+}
+
+__device__ __forceinline__ uint64_t uniform(uint64_t v) {
+  return static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32))) << 32 |
+         __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+}
+
+// 16 bytes per lane from rows + at to LDS, the lanes' pieces one after the other from `to` on.
+__device__ __forceinline__ void load_to_lds(rsrc_t rows, uint32_t at, __attribute__((address_space(3))) void* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rows, to, 16, at, 0, 0, kStreamed);
+}
+
+// Uniform reads through the scalar cache.
+typedef __attribute__((address_space(4))) const int32_t* constant_t;
+__device__ __forceinline__ constant_t constant(const int32_t* p) { return (constant_t)(p); }
+
+// Tokens that a sequence of this length may see, and the units that they take.
+__device__ __forceinline__ uint32_t seen_of(const DecodeParams& p, int32_t len) {
+  const uint32_t n = len < 0 ? 0u : static_cast<uint32_t>(len);
+  return n < p.visible_max ? n : p.visible_max;
+}
+__device__ __forceinline__ uint32_t units_of(const DecodeParams& p, int32_t raw) {
+  const uint32_t len = seen_of(p, raw), start = p.window != 0 && len > p.window ? len - p.window : 0u;
+  return (len - (start & ~(kTile - 1)) + kStep - 1) / kStep;
 }
 
 // One part's statistics of a head. sum < 0 stands for "scores were there, all of them minus
@@ -114,10 +187,13 @@ __device__ __forceinline__ float weight_of(const Stat& s, float top) {
   return s.max == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.max - top);
 }
 
+// Workgroups of a launch, per CU: what is resident at once.
+constexpr uint32_t per_cu(uint32_t dim) { return dim <= 64 ? 4 : dim <= 128 ? 2 : 1; }
+
 // T: queries' type. E4M3: the cache holds that instead. D: head_dim rounded up to 64, 128, 256;
-// EXACT: it is D.
-template <class T, bool E4M3, int D, bool EXACT>
-__global__ __launch_bounds__(kThreads) void decode_kernel(const DecodeParams p) {
+// EXACT: it is D. WHOLE: 16 tokens that start at a multiple of 16 lie within one page.
+template <class T, bool E4M3, int D, bool EXACT, bool WHOLE>
+__global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const DecodeParams p) {
   constexpr int CB = E4M3 ? 1 : 2;                         // bytes of a cached element
   constexpr int KP = D * CB / 64;                          // 16-byte pieces of a K row per lane
   constexpr int VP = D / 16 < 16 / CB ? D / 16 : 16 / CB;  // elements of a V piece
@@ -126,302 +202,501 @@ __global__ __launch_bounds__(kThreads) void decode_kernel(const DecodeParams p) 
   constexpr int NA = NP * VP;                              // accumulators: 16 dims each
   extern __shared__ float lds[];
 
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t col = lane & 15u, kg = lane >> 4;
-  const uint32_t kv_head = blockIdx.x / p.head_tiles, tile = blockIdx.x - kv_head * p.head_tiles;
-  const uint32_t split = blockIdx.y, seq = blockIdx.z;
-  const uint32_t head0 = kv_head * p.group + tile * 16u;
-  const uint32_t n_heads = p.group - tile * 16u < 16u ? p.group - tile * 16u : 16u;
+  const uint32_t team = blockIdx.x / p.rows, member = blockIdx.x - team * p.rows;
   const uint32_t dim = EXACT ? D : p.head_dim;
 
-  // the tokens this sequence sees, and this workgroup's share of them
-  const int32_t raw_len = p.lens[seq];
-  const uint32_t len = raw_len <= 0 ? 0u
-                       : static_cast<uint64_t>(raw_len) < p.visible_max ? static_cast<uint32_t>(raw_len)
-                                                                        : static_cast<uint32_t>(p.visible_max);
-  const uint32_t start = p.window != 0 && len > p.window ? len - p.window : 0u;
-  const uint32_t first = start & ~(kTile - 1);
-  uint32_t chunk = (len - first + p.splits - 1) / p.splits;
-  chunk = (chunk + kStep - 1) / kStep * kStep;
-  if (chunk < p.chunk) chunk = p.chunk;
-  const uint32_t parts = len == 0 ? 1u : (len - first + chunk - 1) / chunk;
-  if (split >= parts) return;
-  const uint32_t begin = first + split * chunk;
-  const uint32_t end = len - begin < chunk ? len : begin + chunk;
-
-  // queries: lane = head, the same numbering of the dims as the pieces of K
-  u32x4 qf[D / 32];
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
-    const uint32_t d = E4M3 ? (c / 2) * 64u + kg * 16u + (c & 1) * 8u : c * 32u + kg * 8u;
-    u32x4 v = {0, 0, 0, 0};
-    if (col < n_heads && (EXACT || d < dim)) {
-      const uint8_t* a = p.q + seq * p.q_token + (head0 + col) * p.q_head + d * 2u;
-      if (p.q_vec) {
-        v = *reinterpret_cast<const u32x4*>(a);
-      } else {
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(a);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = h[2 * j] | static_cast<uint32_t>(h[2 * j + 1]) << 16;
-      }
+  // --- the work: units of kStep tokens, sequence after sequence; team t takes units [t U / n,
+  // (t + 1) U / n) of all U, and each of its workgroups one row (KV head, tiles of its query heads)
+  // of them. Found by every wavefront for itself: lane i adds up the i-th share of the sequences.
+  uint64_t total, before;   // units of all sequences; of those in front of `seq`
+  uint64_t u = 0, u_end = 0;
+  uint32_t n_teams, seq;
+  {
+    const uint32_t each = (p.n_seqs + 63u) / 64u, lanes = (p.n_seqs + each - 1) / each;
+    const uint32_t s0 = lane * each, s1 = s0 + each < p.n_seqs ? s0 + each : p.n_seqs;
+    uint64_t mine = 0;
+    for (uint32_t s = s0; s < s1; ++s) mine += units_of(p, p.lens[s]);
+    uint64_t upto = mine;
+    for (uint32_t d = 1; d < lanes; d *= 2) {
+      const uint64_t other = __shfl_up(upto, d);
+      if (lane >= d) upto += other;
     }
-    qf[c] = v;
+    total = uniform(__shfl(upto, lanes - 1));
+    n_teams = total < p.teams ? static_cast<uint32_t>(total) : p.teams;
+    if (team < n_teams) {
+      u = team * total / n_teams;
+      u_end = (team + 1) * total / n_teams;
+    }
+    uint64_t at = upto - mine;
+    uint32_t s = s0;
+    const bool here = u >= at && u < upto;
+    if (here)
+      for (;; ++s) {
+        const uint32_t n = units_of(p, p.lens[s]);
+        if (u < at + n) break;
+        at += n;
+      }
+    const uint32_t owner = __builtin_ctzll(__ballot(here) | 1ull << 63);
+    seq = __builtin_amdgcn_readlane(s, owner);
+    before = uniform(__shfl(at, owner));
   }
+  const uint64_t u_begin = u;
+
+  // a sequence that sees nothing belongs to no row: zeros
+  for (uint32_t s = blockIdx.x; s < p.n_seqs; s += gridDim.x) {
+    if (seen_of(p, p.lens[s]) != 0) continue;
+    for (uint32_t n = threadIdx.x; n < p.n_heads * dim; n += kThreads) {
+      const uint32_t head = n / dim;
+      reinterpret_cast<uint16_t*>(p.out + s * p.out_token + head * p.out_head)[n - head * dim] = 0;
+    }
+    if (p.lse)
+      for (uint32_t n = threadIdx.x; n < p.n_heads; n += kThreads) p.lse[static_cast<uint64_t>(s) * p.n_heads + n] = -INFINITY;
+  }
+
+  // this workgroup's heads; the wavefronts share them out in tiles of 16 (`spread` tiles side by
+  // side) and then the tokens
+  const uint32_t kv_head = member / p.head_rows, head_row = member - kv_head * p.head_rows;
+  const uint32_t head0 = kv_head * p.group + head_row * p.spread * 16u;
+  const uint32_t left = p.group - head_row * p.spread * 16u;
+  const uint32_t n_heads = left < p.spread * 16u ? left : p.spread * 16u;
+  const uint32_t tile = wave & (p.spread - 1), turn = wave / p.spread;
+  const uint32_t my_heads = n_heads <= tile * 16u ? 0u : n_heads - tile * 16u < 16u ? n_heads - tile * 16u : 16u;
+  const uint32_t step = kStep / p.spread;
 
   const uint8_t* kbase = p.base + kv_head * p.head_stride;
   const uint8_t* vbase = kbase + p.kv_stride;
-  const int32_t* table = p.tables + seq * p.table_stride;
-
-  f32x4 acc[NA];
+  const rsrc_t part_o = rsrc_of(p.part_o), part_ml = rsrc_of(p.part_ml);
+  // K goes through LDS: a load instruction there takes whole rows, one lane after the other 16
+  // bytes, and a row's pieces are stored in an order that lets the 16 rows of a read differ in bank
+  constexpr uint32_t RB = D * CB, PR = RB / 16, RI = 64 / PR, KI = 16 / RI;   // row bytes, pieces; rows per load, loads per half
+  uint8_t* const k_tile = reinterpret_cast<uint8_t*>(lds) + wave * kTile * RB;
+  const auto turned = [](uint32_t row, uint32_t piece) -> uint32_t {
+    return piece ^ ((row / (PR >= 16 ? 1u : 16u / (PR < 16 ? PR : 16u))) & ((PR >= 16 ? 16u : PR) - 1u));
+  };
+  uint32_t k_read[KP];
 #pragma unroll
-  for (int x = 0; x < NA; ++x) acc[x] = f32x4{0, 0, 0, 0};
-  float top = -INFINITY, sum = 0.0f;
-  bool any = false;
-
-  for (uint32_t t0 = begin + wave * kTile; t0 < end; t0 += kStep) {
-    // where the tile's 32 rows lie: lane's column is token col and 16 + col
-    int64_t off[2];
-    uint32_t seen = 0;
+  for (int c = 0; c < KP; ++c)
+    k_read[c] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)(k_tile))) +
+                col * RB + turned(col, c * 4u + kg) * 16u;
+  uint32_t k_lane[KI];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const uint32_t t = t0 + s * 16u + col;
-      bool valid = t >= start && t < end;
-      const uint32_t page = divided(t, p.block_magic);
-      const int32_t block = valid ? table[page] : -1;
-      valid = static_cast<uint32_t>(block) < p.n_blocks;
-      // a token that is not seen reads the cache's first row and takes no part below
-      off[s] = valid ? block * p.block_stride + (t - page * p.ntpb) * p.token_stride : 0;
-      seen |= static_cast<uint32_t>(__ballot(valid) & 0xFFFFu) << (16 * s);
+  for (uint32_t j = 0; j < KI; ++j) {
+    const uint32_t row = j * RI + lane / PR;
+    k_lane[j] = (WHOLE ? row * static_cast<uint32_t>(p.token_stride) : 0u) + turned(row, lane % PR) * 16u;
+  }
+  uint32_t v_lane[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    v_lane[r] = (WHOLE ? (kg * 4 + r) * static_cast<uint32_t>(p.token_stride) : 0u) + col * VP * CB;
+
+  while (u < u_end) {
+    // the sequence that unit u belongs to, and how much of it is this workgroup's
+    const uint32_t len = seen_of(p, constant(p.lens)[seq]);
+    const uint32_t start = p.window != 0 && len > p.window ? len - p.window : 0u;
+    const uint32_t first = start & ~(kTile - 1), units = (len - first + kStep - 1) / kStep;
+    if (u >= before + units) {
+      before += units;
+      ++seq;
+      continue;
     }
-    any = any || seen != 0;
+    const uint32_t unit0 = static_cast<uint32_t>(u - before);
+    const uint32_t n_units = u_end - u < units - unit0 ? static_cast<uint32_t>(u_end - u) : units - unit0;
+    const uint32_t begin = first + unit0 * kStep;
+    const uint32_t end = len - begin < n_units * kStep ? len : begin + n_units * kStep;
 
-    u32x4 kr[2][KP];
+    // queries: lane = head, the same numbering of the dims as the pieces of K
+    u32x4 qf[D / 32];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int c = 0; c < D / 32; ++c) {
+      const uint32_t d = E4M3 ? (c / 2) * 64u + kg * 16u + (c & 1) * 8u : c * 32u + kg * 8u;
+      u32x4 v = {0, 0, 0, 0};
+      if (col < my_heads && (EXACT || d < dim)) {
+        const uint8_t* a = p.q + seq * p.q_token + (head0 + tile * 16u + col) * p.q_head + d * 2u;
+        if (p.q_vec) {
+          v = *reinterpret_cast<const u32x4*>(a);
+        } else {
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(a);
 #pragma unroll
-      for (int c = 0; c < KP; ++c) {
-        const uint32_t at = c * 64u + kg * 16u;
-        kr[s][c] = EXACT || at < dim * CB ? *reinterpret_cast<const u32x4*>(kbase + off[s] + at) : u32x4{0, 0, 0, 0};
+          for (int j = 0; j < 4; ++j) v[j] = h[2 * j] | static_cast<uint32_t>(h[2 * j + 1]) << 16;
+        }
       }
+      qf[c] = v;
+    }
+
+    const int32_t* table = p.tables + seq * p.table_stride;
+    // Block ids of a tile's two halves: one each where a half lies within a page (WHOLE, through
+    // the scalar cache, so that waiting for them is not waiting for rows), else one for the lane's
+    // token of each half. Behind the end the last token's are asked for again.
+    const auto fetch = [&](uint32_t t0, int32_t (&id)[2]) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint32_t t = t0 + s * 16u + (WHOLE ? 0u : col), in = t < len ? t : len - 1;
+        id[s] = WHOLE ? constant(table)[divided(in, p.block_magic)] : table[divided(in, p.block_magic)];
+      }
+    };
+    // ... and where the halves' rows lie: bytes of the half's first row (WHOLE), or of the lane's
+    // token. What is not seen reads some row of the cache and takes no part below. -> seen, a bit each
+    const auto place = [&](uint32_t t0, const int32_t (&id)[2], int64_t (&off)[2]) -> uint32_t {
+      uint32_t seen = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const uint32_t t = t0 + s * 16u + (WHOLE ? 0u : col);
+        bool valid = static_cast<uint32_t>(id[s]) < p.n_blocks;
+        if (!WHOLE) valid = valid && t >= start && t < end;
+        const uint32_t in = t - divided(t, p.block_magic) * p.ntpb;
+        off[s] = valid ? id[s] * p.block_stride + in * p.token_stride : 0;
+        if (WHOLE) {
+          const uint32_t upto = end > t ? (end - t < 16u ? (1u << (end - t)) - 1u : 0xFFFFu) : 0u;
+          const uint32_t from = start > t ? (start - t < 16u ? (1u << (start - t)) - 1u : 0xFFFFu) : 0u;
+          seen |= (valid ? upto & ~from : 0u) << (16 * s);
+        } else {
+          seen |= static_cast<uint32_t>(__ballot(valid) & 0xFFFFu) << (16 * s);
+        }
+      }
+      return seen;
+    };
+    const auto load_k = [&](const int64_t (&off)[2]) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        // (a buffer instruction where it can be: the compiler counts it apart from the loads of V)
+        const rsrc_t rows = rsrc_of(const_cast<uint8_t*>(kbase + (WHOLE ? off[s] : 0)));
+#pragma unroll
+        for (uint32_t j = 0; j < KI; ++j) {
+          const uint32_t row = j * RI + lane / PR;
+          if (EXACT || turned(row, lane % PR) * 16u < dim * CB) {
+            const auto to = (__attribute__((address_space(3))) void*)(k_tile + (s * KI + j) * 1024u);
+            if constexpr (WHOLE)
+              load_to_lds(rows, k_lane[j], to);
+            else
+              __builtin_amdgcn_global_load_lds(
+                  (const __attribute__((address_space(1))) void*)(kbase + __shfl(off[s], row) + k_lane[j]), to, 16, 0, kStreamed);
+          }
+        }
+      }
+    };
+    if (!EXACT) {   // pieces behind the head's end are never written
+      for (uint32_t n = lane; n < kTile * PR; n += 64) reinterpret_cast<u32x4*>(k_tile)[n] = u32x4{0, 0, 0, 0};
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
     // V: the eight tokens whose weights this lane will hold, 4 kg ... + 3 of both halves
     uint32_t vr[8][NP][VW];
+    const auto load_v = [&](const int64_t (&off)[2]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t o = __shfl(off[i >> 2], kg * 4 + (i & 3));
+      for (int i = 0; i < 8; ++i) {
+        const uint8_t* row = vbase + (WHOLE ? off[i >> 2] : __shfl(off[i >> 2], kg * 4 + (i & 3)));
 #pragma unroll
-      for (int h = 0; h < NP; ++h) {
-        const uint32_t d = (h * 16u + col) * VP;
-        const uint8_t* a = vbase + o + d * CB;
-        const bool in = EXACT || d < dim;
-        if constexpr (VW == 4) {
-          const u32x4 v = in ? *reinterpret_cast<const u32x4*>(a) : u32x4{0, 0, 0, 0};
-          vr[i][h][0] = v.x, vr[i][h][1] = v.y, vr[i][h][2] = v.z, vr[i][h][3] = v.w;
-        } else if constexpr (VW == 2) {
-          const u32x2 v = in ? *reinterpret_cast<const u32x2*>(a) : u32x2{0, 0};
-          vr[i][h][0] = v.x, vr[i][h][1] = v.y;
-        } else {
-          vr[i][h][0] = in ? *reinterpret_cast<const uint32_t*>(a) : 0u;
+        for (int h = 0; h < NP; ++h) {
+          const uint8_t* a = row + v_lane[i & 3] + h * 16 * VP * CB;
+          const bool in = EXACT || (h * 16u + col) * VP < dim;
+          if constexpr (VW == 4) {
+            const u32x4 v = in ? streamed<u32x4>(a) : u32x4{0, 0, 0, 0};
+            vr[i][h][0] = v.x, vr[i][h][1] = v.y, vr[i][h][2] = v.z, vr[i][h][3] = v.w;
+          } else if constexpr (VW == 2) {
+            const u32x2 v = in ? streamed<u32x2>(a) : u32x2{0, 0};
+            vr[i][h][0] = v.x, vr[i][h][1] = v.y;
+          } else {
+            vr[i][h][0] = in ? streamed<uint32_t>(a) : 0u;
+          }
         }
       }
-    }
+    };
 
-    // scores
-    f32x4 sc[2];
+    f32x4 acc[NA];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      sc[s] = f32x4{0, 0, 0, 0};
+    for (int x = 0; x < NA; ++x) acc[x] = f32x4{0, 0, 0, 0};
+    float top = -INFINITY, sum = 0.0f;
+    bool any = false;
+
+    // While a tile is worked on, the next one's rows are on their way (K from where this one's
+    // scores are done, V from where its sums are) and the block ids of the one behind.
+    uint32_t t0 = begin + turn * kTile, seen = 0;
+    int32_t id[2];
+    int64_t off[2];
+    const auto work_on = [&](auto more) {
+      constexpr bool MORE = decltype(more)::value;
+      any = any || seen != 0;
+      uint32_t seen_next = 0;
+      if constexpr (MORE) {
+        seen_next = place(t0 + step, id, off);
+        fetch(t0 + 2 * step, id);
+      }
+
+      // scores
+      f32x4 sc[2];
 #pragma unroll
-      for (int c = 0; c < KP; ++c) {
-        if constexpr (E4M3) {
-          const u32x4 w = kr[s][c];
-          const u32x4 a = {T::template widen<false>(w.x), T::template widen<true>(w.x),
-                           T::template widen<false>(w.y), T::template widen<true>(w.y)};
-          const u32x4 b = {T::template widen<false>(w.z), T::template widen<true>(w.z),
-                           T::template widen<false>(w.w), T::template widen<true>(w.w)};
-          sc[s] = T::mma(a, qf[2 * c], sc[s]);
-          sc[s] = T::mma(b, qf[2 * c + 1], sc[s]);
-        } else {
-          sc[s] = T::mma(kr[s][c], qf[c], sc[s]);
+      for (int s = 0; s < 2; ++s) {
+        u32x4 kr[KP];
+        read_k<KP, 8 * NP>(k_read, s * 16 * RB, kr);
+        sc[s] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int c = 0; c < KP; ++c) {
+          if constexpr (E4M3) {
+            const u32x4 w = kr[c];
+            const u32x4 a = {T::template widen<false>(w.x), T::template widen<true>(w.x),
+                             T::template widen<false>(w.y), T::template widen<true>(w.y)};
+            const u32x4 b = {T::template widen<false>(w.z), T::template widen<true>(w.z),
+                             T::template widen<false>(w.w), T::template widen<true>(w.w)};
+            sc[s] = T::mma(a, qf[2 * c], sc[s]);
+            sc[s] = T::mma(b, qf[2 * c + 1], sc[s]);
+          } else {
+            sc[s] = T::mma(kr[c], qf[c], sc[s]);
+          }
         }
       }
-    }
-    float high = -INFINITY;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (MORE) load_k(off);
+      __builtin_amdgcn_sched_barrier(0);
+      if (p.cap != 0.0f) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = sc[s][r] * p.scale_log2;
-        if (p.cap != 0.0f) v = p.cap * tanhf(sc[s][r] * p.cap_in);
-        v = (seen >> (16 * s + 4 * kg + r)) & 1u ? v : -INFINITY;
-        sc[s][r] = v;
-        high = fmaxf(high, v);
+          for (int r = 0; r < 4; ++r) sc[s][r] = p.cap * tanhf(sc[s][r] * p.cap_in);
+      } else {
+        sc[0] *= p.scale_log2;
+        sc[1] *= p.scale_log2;
       }
-    high = fmaxf(over_tokens_max(high), top);
-    if (__any(high != top)) {
-      // a head with nothing but minus infinity so far: exp2(-inf - 0) = 0 below
-      const float shrink = __builtin_amdgcn_exp2f(top - (high == -INFINITY ? 0.0f : high));
-      sum *= shrink;
+      if (seen != 0xFFFFFFFFu) {
+        const uint32_t bits = seen >> (4 * kg);
 #pragma unroll
-      for (int x = 0; x < NA; ++x) acc[x] *= shrink;
-      top = high;
-    }
-    const float ref = high == -INFINITY ? 0.0f : high;
-    u32x4 ph, pl;   // weights cut off, and what that left
+        for (int i = 0; i < 8; ++i)
+          if (!((bits >> (16 * (i >> 2) + (i & 3))) & 1u)) {
+            sc[i >> 2][i & 3] = -INFINITY;
+            // rows that are not seen may hold anything, and zero times anything is not zero
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+            for (int h = 0; h < NP; ++h)
 #pragma unroll
-      for (int r = 0; r < 4; r += 2) {
+              for (int w = 0; w < VW; ++w) vr[i][h][w] = 0;
+          }
+      }
+      float high = top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) high = fmaxf(high, sc[i >> 2][i & 3]);
+      high = over_tokens_max(high);
+      if (__any(high != top)) {
+        // a head with nothing but minus infinity so far: exp2(-inf - 0) = 0
+        const float shrink = __builtin_amdgcn_exp2f(top - (high == -INFINITY ? 0.0f : high));
+        sum *= shrink;
+#pragma unroll
+        for (int x = 0; x < NA; ++x) acc[x] *= shrink;
+        top = high;
+      }
+      const float ref = high == -INFINITY ? 0.0f : high;
+      u32x4 ph, pl;   // weights cut off, and what that left
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = i >> 1, r = 2 * (i & 1);
         const float a = __builtin_amdgcn_exp2f(sc[s][r] - ref), b = __builtin_amdgcn_exp2f(sc[s][r + 1] - ref);
         sum += a + b;
         const uint32_t hi = T::cut(a, b);
         const f32x2 kept = __builtin_convertvector(__builtin_bit_cast(typename T::x2, hi), f32x2);
-        const f32x2 left = {fmaxf(a - kept.x, T::kLeast), fmaxf(b - kept.y, T::kLeast)};
-        ph[s * 2 + r / 2] = hi;
-        pl[s * 2 + r / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(left, typename T::x2));
+        const f32x2 rest = {fmaxf(a - kept.x, T::kLeast), fmaxf(b - kept.y, T::kLeast)};
+        ph[i] = hi;
+        pl[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, typename T::x2));
       }
-
-    if (seen != 0xFFFFFFFFu) {
-      // rows that are not seen may hold anything, and zero times anything is not zero
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (!((seen >> (16 * (i >> 2) + 4 * kg + (i & 3))) & 1u))
+      for (int h = 0; h < NP; ++h)
 #pragma unroll
-          for (int h = 0; h < NP; ++h)
+        for (int w = 0; w < VP / 2; ++w) {   // two dims at a time
+          uint32_t x[8];
 #pragma unroll
-            for (int w = 0; w < VW; ++w) vr[i][h][w] = 0;
-    }
+          for (int i = 0; i < 8; ++i) {
+            if constexpr (E4M3)
+              x[i] = w & 1 ? T::template widen<true>(vr[i][h][w / 2]) : T::template widen<false>(vr[i][h][w / 2]);
+            else
+              x[i] = vr[i][h][w];
+          }
+          u32x4 even, odd;
 #pragma unroll
-    for (int h = 0; h < NP; ++h)
-#pragma unroll
-      for (int w = 0; w < VP / 2; ++w) {   // two dims at a time
-        uint32_t x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if constexpr (E4M3)
-            x[i] = w & 1 ? T::template widen<true>(vr[i][h][w / 2]) : T::template widen<false>(vr[i][h][w / 2]);
-          else
-            x[i] = vr[i][h][w];
+          for (int j = 0; j < 4; ++j) {
+            even[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
+            odd[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
+          }
+          f32x4& a = acc[h * VP + 2 * w];
+          f32x4& b = acc[h * VP + 2 * w + 1];
+          a = T::mma(even, ph, a);
+          b = T::mma(odd, ph, b);
+          a = T::mma(even, pl, a);
+          b = T::mma(odd, pl, b);
         }
-        u32x4 even, odd;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (MORE) load_v(off);
+      __builtin_amdgcn_sched_barrier(0);
+      seen = seen_next;
+    };
+    if (t0 < end && my_heads != 0) {
+      fetch(t0, id);
+      seen = place(t0, id, off);
+      fetch(t0 + step, id);
+      // the queries are here before rows are asked for: waiting for them later would be waiting for
+      // rows too
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          even[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x05040100u);
-          odd[j] = __builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
+      for (int c = 0; c < D / 32; ++c) asm volatile("" : "+v"(qf[c]));
+      load_k(off);
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(off);
+      __builtin_amdgcn_sched_barrier(0);
+      for (; t0 + step < end; t0 += step) work_on(std::true_type());
+      work_on(std::false_type());
+    }
+    __syncthreads();   // no rows of K are in LDS, or on the way there, any more
+
+    // the wavefronts' parts meet in LDS: [wave][head of its tile][dim], rows 4 floats apart from
+    // a multiple of the banks
+    constexpr uint32_t kRow = D + 4;
+    Stat* stats = reinterpret_cast<Stat*>(lds);   // [wave][16]
+    float* part = lds + kWaves * 16 * 2;
+    const uint32_t tile_heads = p.group < 16u ? p.group : 16u;
+    sum = over_tokens_sum(sum);
+    if (sum == 0.0f && any) sum = -1.0f;
+    if (kg == 0) stats[wave * 16 + col] = Stat{top, sum};
+    if (col < my_heads) {
+      float* row = part + (wave * tile_heads + col) * kRow;
+#pragma unroll
+      for (int h = 0; h < NP; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int x = 0; x < VP; x += 4) {
+            const f32x4 v = {acc[h * VP + x][r], acc[h * VP + x + 1][r], acc[h * VP + x + 2][r], acc[h * VP + x + 3][r]};
+            *reinterpret_cast<f32x4*>(row + (h * 16 + kg * 4 + r) * VP + x) = v;
+          }
+    }
+    __syncthreads();
+
+    const uint32_t quads = dim / 4, work = n_heads * quads;
+    const bool whole = n_units == units;
+    const auto finish = [&](uint32_t head, uint32_t d, f32x4 o, float m, float l, bool nothing_but_inf) {
+      const float inv = l == 0.0f ? (nothing_but_inf ? NAN : 0.0f) : p.v_scale / l;
+      uint8_t* a = p.out + seq * p.out_token + (head0 + head) * p.out_head + d * 2u;
+      o *= inv;
+      const f32x2 lo = {o.x, o.y}, hi = {o.z, o.w};
+      const u32x2 w = {__builtin_bit_cast(uint32_t, __builtin_convertvector(lo, typename T::x2)),
+                       __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, typename T::x2))};
+      if (p.out_vec) {
+        *reinterpret_cast<u32x2*>(a) = w;
+      } else {
+        uint16_t* h = reinterpret_cast<uint16_t*>(a);
+        h[0] = w.x, h[1] = w.x >> 16, h[2] = w.y, h[3] = w.y >> 16;
+      }
+      if (d == 0 && p.lse)
+        p.lse[static_cast<uint64_t>(seq) * p.n_heads + head0 + head] =
+            l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    };
+    for (uint32_t n = threadIdx.x; n < work; n += kThreads) {
+      const uint32_t head = n / quads, d = (n - head * quads) * 4;
+      const uint32_t t = head / 16u, h = head - t * 16u;
+      float m = -INFINITY, l = 0.0f;
+      bool inf = false;
+      f32x4 o = {0, 0, 0, 0};
+      for (uint32_t w = t; w < kWaves; w += p.spread) m = fmaxf(m, stats[w * 16 + h].max);
+      for (uint32_t w = t; w < kWaves; w += p.spread) {
+        const Stat s = stats[w * 16 + h];
+        const float f = weight_of(s, m);
+        inf = inf || s.sum < 0.0f;
+        if (f != 0.0f) {
+          l += f * s.sum;
+          o += f * *reinterpret_cast<const f32x4*>(part + (w * tile_heads + h) * kRow + d);
         }
-        f32x4& a = acc[h * VP + 2 * w];
-        f32x4& b = acc[h * VP + 2 * w + 1];
-        a = T::mma(even, ph, a);
-        b = T::mma(odd, ph, b);
-        a = T::mma(even, pl, a);
-        b = T::mma(odd, pl, b);
       }
-  }
-
-  // the four wavefronts' parts meet in LDS: [wave][head][dim], rows 4 floats apart from a
-  // multiple of the banks
-  constexpr uint32_t kRow = D + 4;
-  float* part = lds;
-  Stat* stats = reinterpret_cast<Stat*>(lds + kWaves * n_heads * kRow);   // [wave][16]
-  sum = over_tokens_sum(sum);
-  if (sum == 0.0f && any) sum = -1.0f;
-  if (kg == 0) stats[wave * 16 + col] = Stat{top, sum};
-  if (col < n_heads) {
-    float* row = part + (wave * n_heads + col) * kRow;
+      if (whole) {
+        finish(head, d, o, m, l, inf);
+      } else {
+        const uint32_t at = (2u * blockIdx.x + (u != u_begin)) * p.slot_heads + head;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), part_o, (at * dim + d) * 4u, 0, kShared);
+        if (d == 0)
+          __builtin_amdgcn_raw_buffer_store_b64(
+              u32x2{__float_as_uint(m), __float_as_uint(l == 0.0f && inf ? -1.0f : l)}, part_ml, at * 8u, 0, kShared);
+      }
+    }
+    if (!whole) {
+      // the last workgroup of this row to get here joins the parts, in their order: those of the
+      // teams w0 ... w1, the first's behind whatever it did before
+      const uint32_t w0 = static_cast<uint32_t>(((before + 1) * n_teams - 1) / total);
+      const uint32_t w1 = static_cast<uint32_t>(((before + units) * n_teams - 1) / total);
+      const uint32_t parts = w1 - w0 + 1;
+      const bool behind = w0 * total / n_teams < before;
+      uint32_t* counter = p.counters + w0 * p.rows + member;
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's part is where all can see it
+      __syncthreads();
+      uint32_t* arrived = reinterpret_cast<uint32_t*>(lds);
+      if (threadIdx.x == 0)
+        *arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __syncthreads();
+      const bool last = *arrived == parts - 1;
+      __syncthreads();
+      if (last) {
+        if (threadIdx.x == 0)   // as the next launch on this workspace wants to find it
+          __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const auto slot = [&](uint32_t s) -> uint32_t {
+          return (2u * ((w0 + s) * p.rows + member) + (s == 0 && behind)) * p.slot_heads;
+        };
+        // every float4 of the row by one lane, or by several (crews) that share the parts, kBatch
+        // parts at a time: all asked for at once, then weighed against their maximum
+        constexpr uint32_t kBatch = 8;
+        const uint32_t crews = work < kThreads ? kThreads / work : 1u;
+        for (uint32_t n0 = 0; n0 < work; n0 += kThreads) {
+          const uint32_t crew = work < kThreads ? threadIdx.x / work : 0u;
+          const uint32_t n = work < kThreads ? threadIdx.x - crew * work : n0 + threadIdx.x;
+          const bool active = n < work && crew < crews;
+          const uint32_t head = n / quads, d = (n - head * quads) * 4;
+          float m = -INFINITY, l = 0.0f;
+          bool inf = false;
+          f32x4 o = {0, 0, 0, 0};
+          for (uint32_t s0 = crew; s0 < parts; s0 += kBatch * crews) {
+            u32x2 st[kBatch];
+            u32x4 v[kBatch];
 #pragma unroll
-    for (int h = 0; h < NP; ++h)
+            for (uint32_t k = 0; k < kBatch; ++k) {
+              // a part that is none is behind the buffer's end: zeros come back
+              const uint32_t s = s0 + k * crews, at = slot(s) + head;
+              const bool is = active && s < parts;
+              st[k] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, is ? at * 8u : ~0u, 0, kShared);
+              v[k] = __builtin_amdgcn_raw_buffer_load_b128(part_o, is ? (at * dim + d) * 4u : ~0u, 0, kShared);
+            }
+            float up = m;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+            for (uint32_t k = 0; k < kBatch; ++k) {
+              if (s0 + k * crews >= parts) st[k].x = __float_as_uint(-INFINITY);
+              up = fmaxf(up, __uint_as_float(st[k].x));
+            }
+            const float f_old = weight_of(Stat{m, l}, up);
+            if (f_old != 1.0f) l *= f_old, o *= f_old;
 #pragma unroll
-        for (int x = 0; x < VP; x += 4) {
-          const f32x4 v = {acc[h * VP + x][r], acc[h * VP + x + 1][r], acc[h * VP + x + 2][r], acc[h * VP + x + 3][r]};
-          *reinterpret_cast<f32x4*>(row + (h * 16 + kg * 4 + r) * VP + x) = v;
+            for (uint32_t k = 0; k < kBatch; ++k) {
+              const Stat x = {__uint_as_float(st[k].x), __uint_as_float(st[k].y)};
+              const float f = weight_of(x, up);
+              inf = inf || x.sum < 0.0f;
+              l += f != 0.0f ? f * x.sum : 0.0f;
+              o += f * __builtin_bit_cast(f32x4, v[k]);
+            }
+            m = up;
+          }
+          if (crews > 1) {
+            f32x4* os = reinterpret_cast<f32x4*>(lds);
+            float2* mls = reinterpret_cast<float2*>(lds + kThreads * 4);
+            if (active && crew != 0) {
+              os[threadIdx.x] = o;
+              mls[threadIdx.x] = make_float2(m, l == 0.0f && inf ? -1.0f : l);
+            }
+            __syncthreads();
+            if (active && crew == 0)
+              for (uint32_t t = 1; t < crews; ++t) {
+                const Stat x = {mls[t * work + n].x, mls[t * work + n].y};
+                const float up = fmaxf(m, x.max), f_old = weight_of(Stat{m, l}, up), f = weight_of(x, up);
+                inf = inf || x.sum < 0.0f;
+                if (f_old != 1.0f) l *= f_old, o *= f_old;
+                if (f != 0.0f) l += f * x.sum, o += f * os[t * work + n];
+                m = up;
+              }
+          }
+          if (active && crew == 0) finish(head, d, o, m, l, inf);
         }
-  }
-  __syncthreads();
-
-  const uint32_t quads = dim / 4, work = n_heads * quads;
-  const auto finish = [&](uint32_t head, uint32_t d, f32x4 o, float m, float l, bool nothing_but_inf) {
-    const float inv = l == 0.0f ? (nothing_but_inf ? NAN : 0.0f) : p.v_scale / l;
-    uint8_t* a = p.out + seq * p.out_token + (head0 + head) * p.out_head + d * 2u;
-    o *= inv;
-    const f32x2 lo = {o.x, o.y}, hi = {o.z, o.w};
-    const u32x2 w = {__builtin_bit_cast(uint32_t, __builtin_convertvector(lo, typename T::x2)),
-                     __builtin_bit_cast(uint32_t, __builtin_convertvector(hi, typename T::x2))};
-    if (p.out_vec) {
-      *reinterpret_cast<u32x2*>(a) = w;
-    } else {
-      uint16_t* h = reinterpret_cast<uint16_t*>(a);
-      h[0] = w.x, h[1] = w.x >> 16, h[2] = w.y, h[3] = w.y >> 16;
-    }
-    if (d == 0 && p.lse)
-      p.lse[static_cast<uint64_t>(seq) * p.n_heads + head0 + head] =
-          l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
-  };
-  const uint64_t row0 = (static_cast<uint64_t>(seq) * p.n_heads + head0) * p.splits;
-  for (uint32_t n = threadIdx.x; n < work; n += kThreads) {
-    const uint32_t head = n / quads, d = (n - head * quads) * 4;
-    float m = -INFINITY, l = 0.0f;
-    bool inf = false;
-    f32x4 o = {0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, stats[w * 16 + head].max);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const Stat s = stats[w * 16 + head];
-      const float f = weight_of(s, m);
-      inf = inf || s.sum < 0.0f;
-      if (f != 0.0f) {
-        l += f * s.sum;
-        o += f * *reinterpret_cast<const f32x4*>(part + (w * n_heads + head) * kRow + d);
       }
     }
-    if (parts == 1) {
-      finish(head, d, o, m, l, inf);
-    } else {
-      const uint64_t row = row0 + head * p.splits + split;
-      *reinterpret_cast<f32x4*>(p.part_o + row * dim + d) = o;
-      if (d == 0) p.part_ml[row] = make_float2(m, l == 0.0f && inf ? -1.0f : l);
-    }
-  }
-  if (parts == 1) return;
-
-  // the last workgroup of this group of heads to get here joins the parts, in their order
-  uint32_t* counter = p.counters + static_cast<uint64_t>(seq) * gridDim.x + blockIdx.x;
-  __threadfence();
-  __syncthreads();
-  uint32_t* arrived = reinterpret_cast<uint32_t*>(lds);
-  if (threadIdx.x == 0)
-    *arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  __syncthreads();
-  const bool last = *arrived == parts - 1;
-  if (!last) return;
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) *counter = 0;   // as the next launch on this workspace wants to find it
-  float2* ml = reinterpret_cast<float2*>(lds);   // [head][part]
-  for (uint32_t n = threadIdx.x; n < n_heads * parts; n += kThreads) {
-    const uint32_t head = n / parts, s = n - head * parts;
-    ml[n] = p.part_ml[row0 + head * p.splits + s];
-  }
-  __syncthreads();
-  for (uint32_t n = threadIdx.x; n < work; n += kThreads) {
-    const uint32_t head = n / quads, d = (n - head * quads) * 4;
-    const float2* mine = ml + head * parts;
-    float m = -INFINITY, l = 0.0f;
-    bool inf = false;
-    for (uint32_t s = 0; s < parts; ++s) m = fmaxf(m, mine[s].x);
-    f32x4 o = {0, 0, 0, 0};
-    const float* src = p.part_o + (row0 + head * p.splits) * dim + d;
-    for (uint32_t s = 0; s < parts; ++s) {
-      const Stat st = {mine[s].x, mine[s].y};
-      const float f = weight_of(st, m);
-      inf = inf || st.sum < 0.0f;
-      if (f != 0.0f) {
-        l += f * st.sum;
-        o += f * *reinterpret_cast<const f32x4*>(src + static_cast<uint64_t>(s) * dim);
-      }
-    }
-    finish(head, d, o, m, l, inf);
+    u += n_units;
+    __syncthreads();   // LDS is the next row's
   }
 }
 
@@ -431,12 +706,20 @@ struct Launch {
   hipStream_t stream;
 };
 
+template <class T, bool E4M3, int D, bool EXACT>
+void launch_pages(const DecodeParams& p, const Launch& l) {
+  if (p.ntpb % 16 == 0 && p.token_stride <= (1 << 27))
+    decode_kernel<T, E4M3, D, EXACT, true><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+  else
+    decode_kernel<T, E4M3, D, EXACT, false><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+}
+
 template <class T, bool E4M3, int D>
 void launch_exact(const DecodeParams& p, const Launch& l) {
   if (p.head_dim == D)
-    decode_kernel<T, E4M3, D, true><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+    launch_pages<T, E4M3, D, true>(p, l);
   else
-    decode_kernel<T, E4M3, D, false><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+    launch_pages<T, E4M3, D, false>(p, l);
 }
 
 template <class T, bool E4M3>
@@ -448,12 +731,6 @@ void launch_dim(const DecodeParams& p, const Launch& l) {
   else
     launch_exact<T, E4M3, 256>(p, l);
 }
-
-// Workgroups a split launch aims at: 8 of 4 wavefronts on each of the 256 CUs. A part is at
-// least kMinPart tokens and need not be longer than kMaxPart.
-constexpr uint32_t kAimWgs = 2048, kMinPart = kStep, kMaxPart = 2048;
-// Rows (of one head and part) that a workspace has room for, at most.
-constexpr uint64_t kMaxRowsPerHead = 4096;
 
 }  // namespace
 }  // namespace kvt
@@ -468,9 +745,9 @@ struct kvt_decode {
   int device = 0;
   kvt_kv_layout layout{};
   uint64_t extent = 0;
-  uint32_t dtype = 0, n_heads = 0, group = 0, head_tiles = 0, window = 0, max_seqs = 0;
+  uint32_t dtype = 0, n_heads = 0, group = 0, spread = 0, head_rows = 0, slot_heads = 0, rows = 0, window = 0, max_seqs = 0;
   float scale = 0, cap = 0;
-  uint64_t rows = 0, ws_bytes = 0;
+  uint64_t ws_bytes = 0;
   uint8_t* arena = nullptr;
   struct Owner {
     bool taken = false;
@@ -481,8 +758,9 @@ struct kvt_decode {
   std::mutex mu;
   std::vector<Owner> owners;
 
-  uint64_t ml_at() const { return round_up(rows * layout.head_dim * 4ull, 256); }
-  uint64_t counters_at() const { return round_up(ml_at() + rows * 8ull, 256); }
+  uint32_t n_wgs = 0, teams = 0;
+  uint64_t ml_at() const { return round_up(n_wgs * 2ull * slot_heads * layout.head_dim * 4, 256); }
+  uint64_t counters_at() const { return round_up(ml_at() + n_wgs * 2ull * slot_heads * 8, 256); }
 
   int workspace(hipStream_t s, unsigned long long capture, uint8_t** out) {
     const std::thread::id me = s == hipStreamPerThread ? std::this_thread::get_id() : std::thread::id();
@@ -533,14 +811,18 @@ int kvt_decode_create(int device, const kvt_kv_layout* layout, uint32_t dtype, u
     d->dtype = dtype;
     d->n_heads = n_q_heads;
     d->group = n_q_heads / layout->n_kv_heads;
-    d->head_tiles = (d->group + 15) / 16;
+    const uint32_t tiles = (d->group + 15) / 16;
+    d->spread = tiles >= 3 ? 4 : tiles;
+    d->head_rows = (tiles + d->spread - 1) / d->spread;
+    d->slot_heads = std::min(d->group, 16 * d->spread);
     d->window = window;
     d->max_seqs = max_seqs;
     d->scale = softmax_scale != 0 ? softmax_scale : 1.0f / std::sqrt(static_cast<float>(layout->head_dim));
     d->cap = logit_cap;
-    d->rows = std::min<uint64_t>(kMaxRowsPerHead * std::min(d->group, 16u),
-                                 static_cast<uint64_t>(max_seqs) * n_q_heads * kMaxSplits);
-    const uint64_t counters = static_cast<uint64_t>(max_seqs) * layout->n_kv_heads * d->head_tiles;
+    d->rows = layout->n_kv_heads * d->head_rows;
+    d->teams = std::max(1u, device_cu_count(device) * per_cu(layout->head_dim) / d->rows);
+    d->n_wgs = d->teams * d->rows;
+    const uint64_t counters = d->n_wgs;
     d->ws_bytes = round_up(d->counters_at() + counters * 4, 256);
     d->owners.resize(n_workspaces);
     DeviceGuard g;
@@ -639,9 +921,9 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     p.out = static_cast<uint8_t*>(out), p.out_token = out_token_stride, p.out_head = out_head_stride;
     p.lse = lse;
     p.block_magic = division_magic(d->layout.ntpb);
-    p.visible_max = std::min<uint64_t>(static_cast<uint64_t>(table_blocks) * d->layout.ntpb, 0x7FFFFFFFull);
+    p.visible_max = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(table_blocks) * d->layout.ntpb, 0x7FFFFFFFull));
     p.ntpb = d->layout.ntpb, p.n_blocks = static_cast<uint32_t>(d->layout.n_blocks);
-    p.n_heads = d->n_heads, p.group = d->group, p.head_tiles = d->head_tiles, p.head_dim = dim, p.window = d->window;
+    p.n_heads = d->n_heads, p.group = d->group, p.spread = d->spread, p.head_rows = d->head_rows, p.slot_heads = d->slot_heads, p.head_dim = dim, p.window = d->window;
     const float scale = d->scale * k_scale;
     p.scale_log2 = scale * kLog2e;
     p.cap = d->cap * kLog2e, p.cap_in = d->cap != 0 ? scale / d->cap : 0;
@@ -649,17 +931,13 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     p.q_vec = rows_aligned16(qr);
     p.out_vec = ((reinterpret_cast<uintptr_t>(out) | out_token_stride | out_head_stride) & 7u) == 0;
 
-    // how far to split: max_len is the caller's word and decides nothing but speed
+    p.n_seqs = n_seqs;
+    p.rows = d->rows;
     uint64_t longest = max_len == 0 || max_len > p.visible_max ? p.visible_max : max_len;
-    if (d->window != 0) longest = std::min<uint64_t>(longest, d->window + kTile);
-    const uint64_t groups = static_cast<uint64_t>(d->layout.n_kv_heads) * d->head_tiles;
-    uint64_t chunk = longest * n_seqs * groups / kAimWgs;
-    chunk = round_up(std::min<uint64_t>(std::max<uint64_t>(chunk, kMinPart), kMaxPart), kStep);
-    uint64_t splits = std::max<uint64_t>(1, (longest + chunk - 1) / chunk);
-    splits = std::min<uint64_t>(splits, kMaxSplits);
-    splits = std::max<uint64_t>(1, std::min<uint64_t>(splits, d->rows / (static_cast<uint64_t>(n_seqs) * d->n_heads)));
-    p.chunk = static_cast<uint32_t>(chunk), p.splits = static_cast<uint32_t>(splits);
-    if (splits > 1) {
+    const uint64_t units = (longest + kStep - 1) / kStep * n_seqs;
+    p.teams = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(d->teams, units)));
+    const uint32_t wgs = p.teams * p.rows;
+    {
       uint8_t* ws = nullptr;
       if (int rc = d->workspace(s, capture, &ws)) return rc;
       p.part_o = reinterpret_cast<float*>(ws);
@@ -667,9 +945,9 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
       p.counters = reinterpret_cast<uint32_t*>(ws + d->counters_at());
     }
     const uint32_t heads = std::min(d->group, 16u), full = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-    const uint32_t meet = kWaves * (heads * (full + 4) * 4 + 16 * static_cast<uint32_t>(sizeof(Stat)));
-    const Launch l{dim3(static_cast<uint32_t>(groups), p.splits, n_seqs),
-                   std::max<uint32_t>(meet, splits > 1 ? heads * p.splits * static_cast<uint32_t>(sizeof(float2)) : 0), s};
+    const uint32_t meet = std::max<uint32_t>(kWaves * (heads * (full + 4) * 4 + 16 * static_cast<uint32_t>(sizeof(Stat))),
+                                             kWaves * kTile * full * (e4m3 ? 1 : 2));
+    const Launch l{dim3(wgs), std::max<uint32_t>(meet, kThreads * 24), s};
     if (d->dtype == KVT_DTYPE_BF16) {
       if (e4m3) launch_dim<Bf16, true>(p, l);
       else launch_dim<Bf16, false>(p, l);

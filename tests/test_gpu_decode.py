@@ -112,6 +112,14 @@ def test_head_counts(heads, kv_heads, cache_kind):
     c.check(c.operator(), c.exact())
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(16, 1), (32, 2), (20, 1), (48, 1), (66, 2), (100, 1)])
+@pytest.mark.parametrize("kind,cache_kind,dim", [("bf16", "bf16", 256), ("f16", "e4m3", 256), ("f16", "f16", 144),
+                                                 ("bf16", "bf16", 128)])
+def test_many_heads_of_wide_rows(heads, kv_heads, kind, cache_kind, dim):
+    c = Case(kind, cache_kind, "hnd", [1, 700, 0, 129], heads, kv_heads, dim, 16, seed=19)
+    c.check(c.operator(), c.exact())
+
+
 @pytest.mark.parametrize("dim", [16, 32, 48, 64, 80, 96, 112, 128, 144, 160, 192, 224, 256])
 @pytest.mark.parametrize("kind,cache_kind", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "e4m3")])
 def test_head_sizes(dim, kind, cache_kind):
