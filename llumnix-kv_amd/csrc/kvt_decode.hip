@@ -130,13 +130,21 @@ __device__ __forceinline__ void read_k(const uint32_t* at, int offset, u32x4* r)
 }
 
 // The maximum / sum over the four lanes that hold one head's tokens (lane, +16, +32, +48).
+// Both operands of a swap are the value: what comes back are its even and its odd rows (of 16, of
+// 32 lanes), each in both places.
 __device__ __forceinline__ float over_tokens_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  const uint32_t a = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const uint32_t b = __float_as_uint(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 __device__ __forceinline__ float over_tokens_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  const uint32_t a = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const uint32_t b = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
 }
 
 // Cache policies of the buffer instructions: bit 1 = non-temporal (rows of the cache are read
@@ -150,8 +158,9 @@ __device__ __forceinline__ V streamed(const uint8_t* p) {
 // Parts of split sequences pass from one workgroup to another, on whatever XCD: written through
 // to, and read from, where all XCDs see them (sc1: the scope of the device).
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr uint32_t kNowhere = 0xFFFFF000u;   // the end of every buffer
 __device__ __forceinline__ rsrc_t rsrc_of(void* base) {
-  return __builtin_amdgcn_make_buffer_rsrc(base, 0, 0x7FFFFFFF, 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc(base, 0, kNowhere, 0x00020000);
 }
 
 __device__ __forceinline__ uint64_t uniform(uint64_t v) {
@@ -187,12 +196,15 @@ __device__ __forceinline__ float weight_of(const Stat& s, float top) {
   return s.max == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.max - top);
 }
 
+enum { kWhole, kNear, kFar };
+
 // Workgroups of a launch, per CU: what is resident at once.
 constexpr uint32_t per_cu(uint32_t dim) { return dim <= 64 ? 4 : dim <= 128 ? 2 : 1; }
 
 // T: queries' type. E4M3: the cache holds that instead. D: head_dim rounded up to 64, 128, 256;
-// EXACT: it is D. WHOLE: 16 tokens that start at a multiple of 16 lie within one page.
-template <class T, bool E4M3, int D, bool EXACT, bool WHOLE>
+// EXACT: it is D. PAGES: kWhole where 16 tokens that start at a multiple of 16 lie within one page;
+// else, of a cache whose offsets fit 32 bits, kNear, or kFar.
+template <class T, bool E4M3, int D, bool EXACT, int PAGES>
 __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const DecodeParams p) {
   constexpr int CB = E4M3 ? 1 : 2;                         // bytes of a cached element
   constexpr int KP = D * CB / 64;                          // 16-byte pieces of a K row per lane
@@ -200,6 +212,8 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
   constexpr int NP = D / 16 / VP;                          // V pieces per row and lane
   constexpr int VW = VP * CB / 4;                          // words of a V piece
   constexpr int NA = NP * VP;                              // accumulators: 16 dims each
+  constexpr bool WHOLE = PAGES == kWhole;
+  typedef typename std::conditional<PAGES == kNear, uint32_t, int64_t>::type offset_t;
   extern __shared__ float lds[];
 
   const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -212,12 +226,13 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
   // of them. Found by every wavefront for itself: lane i adds up the i-th share of the sequences.
   uint64_t total, before;   // units of all sequences; of those in front of `seq`
   uint64_t u = 0, u_end = 0;
-  uint32_t n_teams, seq;
+  uint32_t n_teams, seq, len;
   {
     const uint32_t each = (p.n_seqs + 63u) / 64u, lanes = (p.n_seqs + each - 1) / each;
     const uint32_t s0 = lane * each, s1 = s0 + each < p.n_seqs ? s0 + each : p.n_seqs;
     uint64_t mine = 0;
-    for (uint32_t s = s0; s < s1; ++s) mine += units_of(p, p.lens[s]);
+    int32_t raw = 0;   // the length of the last sequence looked at
+    for (uint32_t s = s0; s < s1; ++s) raw = p.lens[s], mine += units_of(p, raw);
     uint64_t upto = mine;
     for (uint32_t d = 1; d < lanes; d *= 2) {
       const uint64_t other = __shfl_up(upto, d);
@@ -232,14 +247,16 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     uint64_t at = upto - mine;
     uint32_t s = s0;
     const bool here = u >= at && u < upto;
-    if (here)
+    if (here && each > 1)
       for (;; ++s) {
-        const uint32_t n = units_of(p, p.lens[s]);
+        raw = p.lens[s];
+        const uint32_t n = units_of(p, raw);
         if (u < at + n) break;
         at += n;
       }
     const uint32_t owner = __builtin_ctzll(__ballot(here) | 1ull << 63);
     seq = __builtin_amdgcn_readlane(s, owner);
+    len = seen_of(p, __builtin_amdgcn_readlane(raw, owner));
     before = uniform(__shfl(at, owner));
   }
   const uint64_t u_begin = u;
@@ -285,20 +302,24 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
   for (uint32_t j = 0; j < KI; ++j) {
     const uint32_t row = j * RI + lane / PR;
     k_lane[j] = (WHOLE ? row * static_cast<uint32_t>(p.token_stride) : 0u) + turned(row, lane % PR) * 16u;
+    // pieces behind the head's end: behind the buffer's end too, so that nothing is read
+    if (!EXACT && turned(row, lane % PR) * 16u >= dim * CB) k_lane[j] = kNowhere;
   }
+  uint32_t v_piece[NP];   // (what dims behind the head's end are read as does not matter)
+#pragma unroll
+  for (uint32_t h = 0; h < NP; ++h) v_piece[h] = EXACT || (h * 16u + col) * VP < dim ? (h * 16u + col) * VP * CB : 0u;
   uint32_t v_lane[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    v_lane[r] = (WHOLE ? (kg * 4 + r) * static_cast<uint32_t>(p.token_stride) : 0u) + col * VP * CB;
+    v_lane[r] = WHOLE ? (kg * 4 + r) * static_cast<uint32_t>(p.token_stride) : 0u;
 
   while (u < u_end) {
     // the sequence that unit u belongs to, and how much of it is this workgroup's
-    const uint32_t len = seen_of(p, constant(p.lens)[seq]);
     const uint32_t start = p.window != 0 && len > p.window ? len - p.window : 0u;
     const uint32_t first = start & ~(kTile - 1), units = (len - first + kStep - 1) / kStep;
     if (u >= before + units) {
       before += units;
-      ++seq;
+      len = seen_of(p, constant(p.lens)[++seq]);
       continue;
     }
     const uint32_t unit0 = static_cast<uint32_t>(u - before);
@@ -338,7 +359,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     };
     // ... and where the halves' rows lie: bytes of the half's first row (WHOLE), or of the lane's
     // token. What is not seen reads some row of the cache and takes no part below. -> seen, a bit each
-    const auto place = [&](uint32_t t0, const int32_t (&id)[2], int64_t (&off)[2]) -> uint32_t {
+    const auto place = [&](uint32_t t0, const int32_t (&id)[2], offset_t (&off)[2]) -> uint32_t {
       uint32_t seen = 0;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
@@ -346,7 +367,10 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
         bool valid = static_cast<uint32_t>(id[s]) < p.n_blocks;
         if (!WHOLE) valid = valid && t >= start && t < end;
         const uint32_t in = t - divided(t, p.block_magic) * p.ntpb;
-        off[s] = valid ? id[s] * p.block_stride + in * p.token_stride : 0;
+        if constexpr (PAGES == kNear)
+          off[s] = valid ? id[s] * static_cast<uint32_t>(p.block_stride) + in * static_cast<uint32_t>(p.token_stride) : 0u;
+        else
+          off[s] = valid ? id[s] * p.block_stride + in * p.token_stride : 0;
         if (WHOLE) {
           const uint32_t upto = end > t ? (end - t < 16u ? (1u << (end - t)) - 1u : 0xFFFFu) : 0u;
           const uint32_t from = start > t ? (start - t < 16u ? (1u << (start - t)) - 1u : 0xFFFFu) : 0u;
@@ -357,7 +381,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       }
       return seen;
     };
-    const auto load_k = [&](const int64_t (&off)[2]) {
+    const auto load_k = [&](const offset_t (&off)[2]) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         // (a buffer instruction where it can be: the compiler counts it apart from the loads of V)
@@ -365,13 +389,15 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
 #pragma unroll
         for (uint32_t j = 0; j < KI; ++j) {
           const uint32_t row = j * RI + lane / PR;
-          if (EXACT || turned(row, lane % PR) * 16u < dim * CB) {
-            const auto to = (__attribute__((address_space(3))) void*)(k_tile + (s * KI + j) * 1024u);
-            if constexpr (WHOLE)
-              load_to_lds(rows, k_lane[j], to);
-            else
-              __builtin_amdgcn_global_load_lds(
-                  (const __attribute__((address_space(1))) void*)(kbase + __shfl(off[s], row) + k_lane[j]), to, 16, 0, kStreamed);
+          const auto to = (__attribute__((address_space(3))) void*)(k_tile + (s * KI + j) * 1024u);
+          if constexpr (PAGES == kWhole) {
+            load_to_lds(rows, k_lane[j], to);
+          } else if constexpr (PAGES == kNear) {
+            const uint32_t at = __shfl(off[s], row) + k_lane[j];
+            load_to_lds(rows, EXACT || k_lane[j] != kNowhere ? at : kNowhere, to);
+          } else if (EXACT || k_lane[j] != kNowhere) {
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)(kbase + __shfl(off[s], row) + k_lane[j]), to, 16, 0, kStreamed);
           }
         }
       }
@@ -382,22 +408,21 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     }
     // V: the eight tokens whose weights this lane will hold, 4 kg ... + 3 of both halves
     uint32_t vr[8][NP][VW];
-    const auto load_v = [&](const int64_t (&off)[2]) {
+    const auto load_v = [&](const offset_t (&off)[2]) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint8_t* row = vbase + (WHOLE ? off[i >> 2] : __shfl(off[i >> 2], kg * 4 + (i & 3)));
 #pragma unroll
         for (int h = 0; h < NP; ++h) {
-          const uint8_t* a = row + v_lane[i & 3] + h * 16 * VP * CB;
-          const bool in = EXACT || (h * 16u + col) * VP < dim;
+          const uint8_t* a = row + v_lane[i & 3] + v_piece[h];
           if constexpr (VW == 4) {
-            const u32x4 v = in ? streamed<u32x4>(a) : u32x4{0, 0, 0, 0};
+            const u32x4 v = streamed<u32x4>(a);
             vr[i][h][0] = v.x, vr[i][h][1] = v.y, vr[i][h][2] = v.z, vr[i][h][3] = v.w;
           } else if constexpr (VW == 2) {
-            const u32x2 v = in ? streamed<u32x2>(a) : u32x2{0, 0};
+            const u32x2 v = streamed<u32x2>(a);
             vr[i][h][0] = v.x, vr[i][h][1] = v.y;
           } else {
-            vr[i][h][0] = in ? streamed<uint32_t>(a) : 0u;
+            vr[i][h][0] = streamed<uint32_t>(a);
           }
         }
       }
@@ -413,7 +438,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     // scores are done, V from where its sums are) and the block ids of the one behind.
     uint32_t t0 = begin + turn * kTile, seen = 0;
     int32_t id[2];
-    int64_t off[2];
+    offset_t off[2];
     const auto work_on = [&](auto more) {
       constexpr bool MORE = decltype(more)::value;
       any = any || seen != 0;
@@ -632,67 +657,88 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
         const auto slot = [&](uint32_t s) -> uint32_t {
           return (2u * ((w0 + s) * p.rows + member) + (s == 0 && behind)) * p.slot_heads;
         };
-        // every float4 of the row by one lane, or by several (crews) that share the parts, kBatch
-        // parts at a time: all asked for at once, then weighed against their maximum
-        constexpr uint32_t kBatch = 8;
-        const uint32_t crews = work < kThreads ? kThreads / work : 1u;
-        for (uint32_t n0 = 0; n0 < work; n0 += kThreads) {
-          const uint32_t crew = work < kThreads ? threadIdx.x / work : 0u;
-          const uint32_t n = work < kThreads ? threadIdx.x - crew * work : n0 + threadIdx.x;
-          const bool active = n < work && crew < crews;
-          const uint32_t head = n / quads, d = (n - head * quads) * 4;
-          float m = -INFINITY, l = 0.0f;
-          bool inf = false;
-          f32x4 o = {0, 0, 0, 0};
-          for (uint32_t s0 = crew; s0 < parts; s0 += kBatch * crews) {
-            u32x2 st[kBatch];
-            u32x4 v[kBatch];
+        // Q float4s of a head by one lane, or by several (crews) that share the parts; kBatch parts
+        // at a time, all asked for at once, then weighed against their maximum. Two where that saves
+        // a pass (32 heads of 192, 21 parts: 35 -> 28 us for the launch), else one, whose crews have
+        // less to tell one another.
+        const auto join = [&](auto quads_each) {
+          constexpr uint32_t Q = decltype(quads_each)::value, kBatch = 8;
+          const uint32_t per_head = dim / (4 * Q), jobs = n_heads * per_head;
+          const uint32_t crews = jobs < kThreads ? kThreads / jobs : 1u;
+          for (uint32_t n0 = 0; n0 < jobs; n0 += kThreads) {
+            const uint32_t crew = jobs < kThreads ? threadIdx.x / jobs : 0u;
+            const uint32_t n = jobs < kThreads ? threadIdx.x - crew * jobs : n0 + threadIdx.x;
+            const bool active = n < jobs && crew < crews;
+            const uint32_t head = n / per_head, d = (n - head * per_head) * (4 * Q);
+            float m = -INFINITY, l = 0.0f;
+            bool inf = false;
+            f32x4 o[Q] = {};
+            for (uint32_t s0 = crew; s0 < parts; s0 += kBatch * crews) {
+              u32x2 st[kBatch];
+              u32x4 v[kBatch][Q];
 #pragma unroll
-            for (uint32_t k = 0; k < kBatch; ++k) {
-              // a part that is none is behind the buffer's end: zeros come back
-              const uint32_t s = s0 + k * crews, at = slot(s) + head;
-              const bool is = active && s < parts;
-              st[k] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, is ? at * 8u : ~0u, 0, kShared);
-              v[k] = __builtin_amdgcn_raw_buffer_load_b128(part_o, is ? (at * dim + d) * 4u : ~0u, 0, kShared);
-            }
-            float up = m;
+              for (uint32_t k = 0; k < kBatch; ++k) {
+                // a part that is none is behind the buffer's end: zeros come back
+                const uint32_t s = s0 + k * crews, at = slot(s) + head;
+                const bool is = active && s < parts;
+                st[k] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, is ? at * 8u : kNowhere, 0, kShared);
 #pragma unroll
-            for (uint32_t k = 0; k < kBatch; ++k) {
-              if (s0 + k * crews >= parts) st[k].x = __float_as_uint(-INFINITY);
-              up = fmaxf(up, __uint_as_float(st[k].x));
-            }
-            const float f_old = weight_of(Stat{m, l}, up);
-            if (f_old != 1.0f) l *= f_old, o *= f_old;
-#pragma unroll
-            for (uint32_t k = 0; k < kBatch; ++k) {
-              const Stat x = {__uint_as_float(st[k].x), __uint_as_float(st[k].y)};
-              const float f = weight_of(x, up);
-              inf = inf || x.sum < 0.0f;
-              l += f != 0.0f ? f * x.sum : 0.0f;
-              o += f * __builtin_bit_cast(f32x4, v[k]);
-            }
-            m = up;
-          }
-          if (crews > 1) {
-            f32x4* os = reinterpret_cast<f32x4*>(lds);
-            float2* mls = reinterpret_cast<float2*>(lds + kThreads * 4);
-            if (active && crew != 0) {
-              os[threadIdx.x] = o;
-              mls[threadIdx.x] = make_float2(m, l == 0.0f && inf ? -1.0f : l);
-            }
-            __syncthreads();
-            if (active && crew == 0)
-              for (uint32_t t = 1; t < crews; ++t) {
-                const Stat x = {mls[t * work + n].x, mls[t * work + n].y};
-                const float up = fmaxf(m, x.max), f_old = weight_of(Stat{m, l}, up), f = weight_of(x, up);
-                inf = inf || x.sum < 0.0f;
-                if (f_old != 1.0f) l *= f_old, o *= f_old;
-                if (f != 0.0f) l += f * x.sum, o += f * os[t * work + n];
-                m = up;
+                for (uint32_t x = 0; x < Q; ++x)
+                  v[k][x] = __builtin_amdgcn_raw_buffer_load_b128(part_o, is ? (at * dim + d) * 4u + x * 16u : kNowhere, 0, kShared);
               }
+              float up = m;
+#pragma unroll
+              for (uint32_t k = 0; k < kBatch; ++k) {
+                if (s0 + k * crews >= parts) st[k].x = __float_as_uint(-INFINITY);
+                up = fmaxf(up, __uint_as_float(st[k].x));
+              }
+              const float f_old = weight_of(Stat{m, l}, up);
+              if (f_old != 1.0f) {
+                l *= f_old;
+#pragma unroll
+                for (uint32_t x = 0; x < Q; ++x) o[x] *= f_old;
+              }
+#pragma unroll
+              for (uint32_t k = 0; k < kBatch; ++k) {
+                const Stat part_st = {__uint_as_float(st[k].x), __uint_as_float(st[k].y)};
+                const float f = weight_of(part_st, up);
+                inf = inf || part_st.sum < 0.0f;
+                l += f != 0.0f ? f * part_st.sum : 0.0f;
+#pragma unroll
+                for (uint32_t x = 0; x < Q; ++x) o[x] += f * __builtin_bit_cast(f32x4, v[k][x]);
+              }
+              m = up;
+            }
+            if (crews > 1) {
+              f32x4* os = reinterpret_cast<f32x4*>(lds);
+              Stat* mls = reinterpret_cast<Stat*>(lds + kThreads * 4 * Q);
+              if (active && crew != 0) {
+#pragma unroll
+                for (uint32_t x = 0; x < Q; ++x) os[Q * threadIdx.x + x] = o[x];
+                mls[threadIdx.x] = Stat{m, l == 0.0f && inf ? -1.0f : l};
+              }
+              __syncthreads();
+              if (active && crew == 0)
+                for (uint32_t t = 1; t < crews; ++t) {
+                  const uint32_t at = t * jobs + n;
+                  const Stat other = mls[at];
+                  const float up = fmaxf(m, other.max), f_old = weight_of(Stat{m, l}, up), f = weight_of(other, up);
+                  inf = inf || other.sum < 0.0f;
+                  l = (f_old != 0.0f ? f_old * l : 0.0f) + (f != 0.0f ? f * other.sum : 0.0f);
+#pragma unroll
+                  for (uint32_t x = 0; x < Q; ++x) o[x] = (f_old != 0.0f ? f_old : 0.0f) * o[x] + f * os[Q * at + x];
+                  m = up;
+                }
+            }
+            if (active && crew == 0)
+#pragma unroll
+              for (uint32_t x = 0; x < Q; ++x) finish(head, d + 4 * x, o[x], m, l, inf);
           }
-          if (active && crew == 0) finish(head, d, o, m, l, inf);
-        }
+        };
+        if (D > 64 && work >= kThreads)
+          join(std::integral_constant<uint32_t, D == 64 ? 1 : 2>());
+        else
+          join(std::integral_constant<uint32_t, 1>());
       }
     }
     u += n_units;
@@ -703,15 +749,18 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
 struct Launch {
   dim3 grid;
   uint32_t lds;
+  int pages;
   hipStream_t stream;
 };
 
 template <class T, bool E4M3, int D, bool EXACT>
 void launch_pages(const DecodeParams& p, const Launch& l) {
-  if (p.ntpb % 16 == 0 && p.token_stride <= (1 << 27))
-    decode_kernel<T, E4M3, D, EXACT, true><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+  if (l.pages == kWhole)
+    decode_kernel<T, E4M3, D, EXACT, kWhole><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+  else if (l.pages == kNear)
+    decode_kernel<T, E4M3, D, EXACT, kNear><<<l.grid, kThreads, l.lds, l.stream>>>(p);
   else
-    decode_kernel<T, E4M3, D, EXACT, false><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+    decode_kernel<T, E4M3, D, EXACT, kFar><<<l.grid, kThreads, l.lds, l.stream>>>(p);
 }
 
 template <class T, bool E4M3, int D>
@@ -947,7 +996,10 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     const uint32_t heads = std::min(d->group, 16u), full = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     const uint32_t meet = std::max<uint32_t>(kWaves * (heads * (full + 4) * 4 + 16 * static_cast<uint32_t>(sizeof(Stat))),
                                              kWaves * kTile * full * (e4m3 ? 1 : 2));
-    const Launch l{dim3(wgs), std::max<uint32_t>(meet, kThreads * 24), s};
+    const int pages = d->layout.ntpb % 16 == 0 && d->layout.token_stride <= (1u << 27) ? kWhole
+                      : d->extent < kNowhere                                          ? kNear
+                                                                                      : kFar;
+    const Launch l{dim3(wgs), std::max<uint32_t>(meet, kThreads * 40), pages, s};
     if (d->dtype == KVT_DTYPE_BF16) {
       if (e4m3) launch_dim<Bf16, true>(p, l);
       else launch_dim<Bf16, false>(p, l);

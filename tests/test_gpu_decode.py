@@ -265,10 +265,49 @@ def test_long_sequences_split_over_the_device():
             assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
-def test_many_short_sequences():
+@pytest.mark.parametrize("n", [63, 64, 65, 700])
+def test_many_short_sequences(n):
     rng = np.random.default_rng(12)
-    c = Case("bf16", "bf16", "flash", rng.integers(0, 70, 700), 4, 2, 64, 16, seed=12)
+    c = Case("bf16", "bf16", "flash", rng.integers(0, 70, n), 4, 2, 64, 16, seed=12)
     c.check(c.operator(max_seqs=1000), c.exact(), max_len=70)
+
+
+def test_uneven_sequences_in_many_shares():
+    """More sequences than a wavefront has lanes, one much longer than the rest, empty ones in front,
+    between and behind: shares that begin and end anywhere."""
+    lens = [0, 0, 5] + [0, 40, 129, 0] * 30 + [9000] + [1, 0, 128] * 25 + [0, 0]
+    for kv, heads, dim in ((1, 4, 64), (3, 9, 128)):
+        c = Case("bf16", "bf16", "hnd", lens, heads, kv, dim, 16, seed=20)
+        op, exact = c.operator(), c.exact()
+        first = c.check(op, exact)
+        for max_len in (1, 300):
+            c.check(op, exact, max_len=max_len)
+        again = c.check(op, exact)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_pages_of_a_cache_beyond_32_bits_that_end_inside_a_tile():
+    """Offsets that need 64 bits and block sizes that are no multiple of 16: a cache of 5 GiB."""
+    block, kv, dim = 5, 1, 256
+    n_blocks = (5 << 30) // (2 * block * kv * dim * 2)
+    cache = torch.zeros((n_blocks, 2, block, kv, dim), device="cuda", dtype=torch.bfloat16)
+    handle = kvt_amd.Cache(0, [[cache]], [cache.numel() * 2])
+    lay = kvt_amd.KvLayout(kvt_amd.SHAPE_QWEN3_NEXT_FLASH, "bf16", n_blocks, block, kv, dim)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(21)
+    ids = np.array([n_blocks - 1, 0, n_blocks - 7] + list(range(n_blocks // 2, n_blocks // 2 + 60)), dtype=np.int64)
+    n = block * len(ids) - 2
+    k, v, q = (torch.randn((m, h, dim), generator=g, device="cuda").to(torch.bfloat16)
+               for m, h in ((n, kv), (n, kv), (1, 4)))
+    kvt_amd.kv_append(handle, 0, lay, k, v, torch.from_numpy(ids[np.arange(n) // block] * block + np.arange(n) % block).cuda())
+    out, lse = torch.empty_like(q), torch.empty((1, 4), device="cuda")
+    op = kvt_amd.DecodeAttention(0, lay, "bf16", 4, max_seqs=1)
+    op.run(handle, 0, q, torch.from_numpy(ids.astype(np.int32)[None]).cuda(),
+           torch.tensor([n], dtype=torch.int32, device="cuda"), out, lse=lse)
+    pad = ((0, 2), (0, 0), (0, 0))
+    exact = oc.decode_exact(oc.wide(q), *(np.pad(oc.wide(x), pad).reshape(len(ids), block, kv, dim) for x in (k, v)),
+                            np.arange(len(ids))[None], [n], block, dim ** -0.5)
+    hold(out, lse, exact, "bf16")
 
 
 def test_offsets_beyond_32_bits():
