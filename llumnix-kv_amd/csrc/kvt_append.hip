@@ -1,11 +1,12 @@
 // Rotary positions, and the append of a step's keys and values to the paged cache.
 //
-// Both are one kernel over a flat list of items. An item is what a lane moves: of a rotated row
-// 2 N elements that hold N whole pairs (half layout: N at u and N at rotary_dim / 2 + u;
-// interleaved: 2 N in a row), of everything else N elements, N = 16 bytes' worth (or 1 where an
-// alignment forbids vectors). The items of a token -- its query rows, key rows, value rows --
-// follow one another, and so do the tokens, so that every lane of every workgroup has work
-// whatever the head counts are.
+// Both are one kernel over a flat list of items. An item is what a lane moves: two pieces of a
+// row, N = 16 bytes' worth of elements each (or 1 where an alignment forbids vectors). Of a rotated
+// part in the half layout they are the two sides of N pairs; everywhere else the i-th piece of the
+// part's first half and the i-th of its second, which leaves every load and store 16 bytes a lane,
+// lanes side by side. The items of a token -- its query rows, key rows, value rows -- follow one
+// another, and so do the tokens, so that every lane of every workgroup has work whatever the head
+// counts are.
 //
 // The angle position * frequency is formed in 64 bits, in turns, and reduced there to the nearest
 // quarter: a product in 32 bits would be off by 2^-24 of the angle, half a radian at position
@@ -25,7 +26,13 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256;
-constexpr uint32_t kItemsPerLane = 2;
+constexpr uint32_t kItemsPerLane = 1;
+// Stores are non-temporal. Loads are so where the launch reads more than this: less is still in the
+// 256 MiB memory-side cache after the projection that made it. Microseconds a call, heads of 32 + 8
+// + 8 x 128 bf16, all plain / plain loads, non-temporal stores / both non-temporal: 2048 tokens
+// (25 MB read) 9.6 / 9.0 / 10.2, 4096 18.8 / 15.9 / 18.4, 8192 38.0 / 33.4 / 34.1, 16384 (201 MB)
+// 73.9 / 69.8 / 66.4.
+constexpr uint64_t kCachedInput = 128ull << 20;
 constexpr uint32_t kItemsPerWg = kThreads * kItemsPerLane;
 
 struct RotateParams {
@@ -37,14 +44,27 @@ struct RotateParams {
   int64_t block_stride, kv_stride, token_stride, head_stride;
   const int64_t *positions, *slots;
   uint64_t n_tokens, n_slots;
-  uint64_t items_magic, row_magic, v_row_magic, half_magic, block_magic;
+  uint64_t items_magic, row_magic, half_magic, block_magic;
   uint32_t items, q_items, qk_items;   // per token: all, of the queries, of queries and keys
-  uint32_t row_items, v_row_items;     // per rotated row, per value row
-  uint32_t rot_items;                  // the rotated ones of a rotated row, in front
-  uint32_t half, ntpb;                 // pairs per row
+  uint32_t row_items, rot_items;       // per row; of a query or key row, the rotated ones in front
+  uint32_t half, dim, ntpb;            // pairs and elements of a row
+  bool near;                           // all items of the launch are fewer than 2^32
+  bool once;                           // for the launcher: more is read than kCachedInput
   float k_mul, v_mul, magnitude;
-  double turns[128];
 };
+
+// The frequencies travel with the launch; 64 of them (heads of 128) where they are enough, since
+// a launch's arguments cost host time by their size (a rotary call: 5.3 us with room for 128, 4.2 with 64).
+template <int PAIRS>
+struct Turns {
+  double per_position[PAIRS];
+};
+
+// Every pointer here is to global memory, also where the compiler cannot tell.
+template <class V, class P>
+__device__ __forceinline__ __attribute__((address_space(1))) V* global(P* p) {
+  return (__attribute__((address_space(1))) V*)(p);
+}
 
 struct Bf16 {
   static __device__ __forceinline__ float wide(uint32_t bits) { return __uint_as_float(bits << 16); }
@@ -86,25 +106,27 @@ struct Piece {
   static constexpr int kWords = N == 1 ? 1 : N * kElem / 4;
   uint32_t w[kWords];
 
+  template <bool ONCE>
   __device__ __forceinline__ void load(const uint8_t* p) {
     if constexpr (N == 1) {
       if constexpr (kElem == 4)
-        w[0] = *reinterpret_cast<const uint32_t*>(p);
+        w[0] = *global<const uint32_t>(p);
       else
-        w[0] = *reinterpret_cast<const uint16_t*>(p);
+        w[0] = *global<const uint16_t>(p);
     } else {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+      const auto at = global<const u32x4>(p);
+      const u32x4 v = ONCE ? __builtin_nontemporal_load(at) : *at;
       w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
     }
   }
   __device__ __forceinline__ void store(uint8_t* p) const {
     if constexpr (N == 1) {
       if constexpr (kElem == 4)
-        *reinterpret_cast<uint32_t*>(p) = w[0];
+        *global<uint32_t>(p) = w[0];
       else
-        *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[0]);
+        *global<uint16_t>(p) = static_cast<uint16_t>(w[0]);
     } else {
-      *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+      __builtin_nontemporal_store((u32x4{w[0], w[1], w[2], w[3]}), global<u32x4>(p));
     }
   }
   __device__ __forceinline__ void widen(float* f) const {
@@ -136,10 +158,12 @@ __device__ __forceinline__ void store_e4m3(uint8_t* p, const float* f) {
     u32x2 r;
     r.x = to_e4m3<true>(f[2], f[3], to_e4m3<false>(f[0], f[1], 0u));
     r.y = to_e4m3<true>(f[6], f[7], to_e4m3<false>(f[4], f[5], 0u));
-    *reinterpret_cast<u32x2*>(p) = r;
+
+    __builtin_nontemporal_store(r, global<u32x2>(p));
+
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) p[i] = static_cast<uint8_t>(to_e4m3<false>(f[i], 0.0f, 0u));
+    for (int i = 0; i < N; ++i) *global<uint8_t>(p + i) = static_cast<uint8_t>(to_e4m3<false>(f[i], 0.0f, 0u));
   }
 }
 
@@ -148,20 +172,21 @@ template <class T, int N>
 struct Item {
   Piece<T, N> a, b;
   uint8_t* out;           // where the row starts; nullptr: no item, or a slot that is none
-  uint32_t at_a, at_b;    // elements into the row
+  uint32_t at_a, at_b;    // elements into the row; at_b == 0: there is no second piece
   uint32_t angle;         // first pair's place in the workgroup's table
   float mul;              // of the cache's scale
   bool rotated, narrow;   // narrow: to the cache's 8-bit type
 };
 
 // T: type of queries, keys and values. E4M3: the cache holds that instead of T. N: elements of
-// a piece. INTER: pairs lie next to each other.
-template <class T, bool E4M3, int N, bool INTER>
-__global__ __launch_bounds__(kThreads) void rotate_append_kernel(const RotateParams p) {
+// a piece. INTER: pairs lie next to each other. PAIRS: room for frequencies. ONCE: read with
+// non-temporal loads.
+template <class T, bool E4M3, int N, bool INTER, int PAIRS, bool ONCE>
+__global__ __launch_bounds__(kThreads) void rotate_append_kernel(const RotateParams p, const Turns<PAIRS> turns) {
   extern __shared__ float2 cs[];
   constexpr int kElem = Piece<T, N>::kElem;
   const uint64_t first = static_cast<uint64_t>(blockIdx.x) * kItemsPerWg;
-  const uint64_t token0 = first / p.items;
+  const uint64_t token0 = p.near ? divided(static_cast<uint32_t>(first), p.items_magic) : first / p.items;
   const uint32_t rem = static_cast<uint32_t>(first - token0 * p.items);
 
   Item<T, N> it[kItemsPerLane];
@@ -174,52 +199,40 @@ __global__ __launch_bounds__(kThreads) void rotate_append_kernel(const RotatePar
     const uint64_t t = token0 + tl;
     if (t >= p.n_tokens) continue;
     uint32_t i = f - tl * p.items;
-    const uint8_t* in;
-    const bool to_cache = i >= p.q_items;
+    const bool to_cache = i >= p.q_items, value = i >= p.qk_items;
+    i -= value ? p.qk_items : to_cache ? p.q_items : 0u;
+    const uint32_t row = divided(i, p.row_magic), u = i - row * p.row_items;
+    x.rotated = !value && u < p.rot_items;
     x.narrow = E4M3 && to_cache;
-    if (i < p.qk_items) {
-      if (to_cache) i -= p.q_items;
-      const uint32_t row = divided(i, p.row_magic);
-      const uint32_t u = i - row * p.row_items;
-      x.rotated = u < p.rot_items;
-      if (!x.rotated) {
-        x.at_a = x.at_b = 2 * p.half + (u - p.rot_items) * N;
-      } else if constexpr (INTER) {
-        x.at_a = 2 * u * N, x.at_b = x.at_a + N;
-      } else {
-        x.at_a = u * N, x.at_b = x.at_a + p.half;
-      }
-      x.angle = tl * p.half + u * N;
-      if (to_cache) {
-        in = p.k + t * p.k_token + row * p.k_head;
-        x.out = p.cache + row * p.head_stride;
-        x.mul = p.k_mul;
-      } else {
-        in = p.q + t * p.q_token + row * p.q_head;
-        x.out = p.q_out + t * p.q_out_token + row * p.q_out_head;
-        x.mul = 1.0f;
-      }
+    if (x.rotated) {
+      x.at_a = INTER && N == 1 ? 2 * u : u * N;
+      x.at_b = INTER && N == 1 ? 2 * u + 1 : p.half + u * N;
+      // the first pair of the item (of each piece, where a piece holds its pairs whole)
+      x.angle = tl * p.half + (INTER && N > 1 ? u * N / 2 : u * N);
     } else {
-      i -= p.qk_items;
-      const uint32_t row = divided(i, p.v_row_magic);
-      x.at_a = x.at_b = (i - row * p.v_row_items) * N;
-      x.rotated = false;
-      x.mul = p.v_mul;
-      in = p.v + t * p.v_token + row * p.v_head;
-      x.out = p.cache + p.kv_stride + row * p.head_stride;
+      const uint32_t front = value ? 0u : 2 * p.half, rest = p.dim - front;
+      const uint32_t v = value ? u : u - p.rot_items;
+      x.at_a = front + v * N;
+      x.at_b = x.at_a + (rest + 1) / 2;
+      if (N == 1 && x.at_b >= p.dim) x.at_b = 0;   // the middle one of an odd number
     }
-    if (to_cache) {   // a slot that is none (padding) has no row
+    const uint8_t* in;
+    if (to_cache) {
+      in = value ? p.v + t * p.v_token + row * p.v_head : p.k + t * p.k_token + row * p.k_head;
+      x.mul = value ? p.v_mul : p.k_mul;
       const uint64_t slot = static_cast<uint64_t>(p.slots[t]);
-      if (slot >= p.n_slots) {
-        x.out = nullptr;
-        continue;
-      }
+      if (slot >= p.n_slots) continue;   // none (padding): no row
       const uint64_t block =
           p.n_slots <= 0xFFFFFFFFull ? divided(static_cast<uint32_t>(slot), p.block_magic) : slot / p.ntpb;
-      x.out += block * p.block_stride + (slot - block * p.ntpb) * p.token_stride;
+      x.out = p.cache + block * p.block_stride + (slot - block * p.ntpb) * p.token_stride + row * p.head_stride +
+              (value ? p.kv_stride : 0);
+    } else {
+      in = p.q + t * p.q_token + row * p.q_head;
+      x.out = p.q_out + t * p.q_out_token + row * p.q_out_head;
+      x.mul = 1.0f;
     }
-    x.a.load(in + x.at_a * kElem);
-    if (x.rotated) x.b.load(in + x.at_b * kElem);
+    x.a.template load<ONCE>(in + x.at_a * kElem);
+    if (N > 1 || x.at_b != 0) x.b.template load<ONCE>(in + x.at_b * kElem);
   }
 
   if (p.half != 0) {
@@ -228,7 +241,7 @@ __global__ __launch_bounds__(kThreads) void rotate_append_kernel(const RotatePar
     const uint32_t tokens = left < span ? static_cast<uint32_t>(left) : span;
     for (uint32_t n = threadIdx.x; n < tokens * p.half; n += kThreads) {
       const uint32_t tl = divided(n, p.half_magic);
-      double turn = static_cast<double>(p.positions[token0 + tl]) * p.turns[n - tl * p.half];
+      double turn = static_cast<double>(p.positions[token0 + tl]) * turns.per_position[n - tl * p.half];
       turn -= rint(turn);
       const double quarter = rint(4.0 * turn);
       float s, c;
@@ -245,54 +258,72 @@ __global__ __launch_bounds__(kThreads) void rotate_append_kernel(const RotatePar
   for (uint32_t n = 0; n < kItemsPerLane; ++n) {
     Item<T, N>& x = it[n];
     if (!x.out) continue;
-    if (x.rotated) {
-      float a[2 * N], r[2 * N];
+    if (x.rotated || (E4M3 && x.narrow)) {
+      float a[2 * N];
       x.a.widen(a);
-      x.b.widen(a + N);
+      if (N > 1 || x.at_b != 0) x.b.widen(a + N);
+      if (x.rotated) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int i0 = INTER ? 2 * j : j, i1 = INTER ? 2 * j + 1 : N + j;
-        const float2 t = cs[x.angle + j];
-        r[i0] = a[i0] * t.x - a[i1] * t.y;
-        r[i1] = a[i0] * t.y + a[i1] * t.x;
+        for (int j = 0; j < N; ++j) {
+          // pair j of the item: across its two pieces, or within one of them
+          constexpr bool kWithin = INTER && N > 1;
+          const int i0 = kWithin ? 2 * j : j, i1 = kWithin ? 2 * j + 1 : N + j;
+          const uint32_t at = kWithin && j >= N / 2 ? x.angle + p.half / 2 + j - N / 2 : x.angle + j;
+          const float2 t = cs[at];
+          const float x0 = a[i0], x1 = a[i1];
+          a[i0] = x0 * t.x - x1 * t.y;
+          a[i1] = x0 * t.y + x1 * t.x;
+        }
       }
       if (E4M3 && x.narrow) {
 #pragma unroll
-        for (int j = 0; j < 2 * N; ++j) r[j] *= x.mul;
-        store_e4m3<N>(x.out + x.at_a, r);
-        store_e4m3<N>(x.out + x.at_b, r + N);
-      } else {
-        x.a.round(r);
-        x.b.round(r + N);
-        x.a.store(x.out + x.at_a * kElem);
-        x.b.store(x.out + x.at_b * kElem);
+        for (int j = 0; j < 2 * N; ++j) a[j] *= x.mul;
+        store_e4m3<N>(x.out + x.at_a, a);
+        if (N > 1 || x.at_b != 0) store_e4m3<N>(x.out + x.at_b, a + N);
+        continue;
       }
-    } else if (E4M3 && x.narrow) {
-      float a[N];
-      x.a.widen(a);
-#pragma unroll
-      for (int j = 0; j < N; ++j) a[j] *= x.mul;
-      store_e4m3<N>(x.out + x.at_a, a);
-    } else {
-      x.a.store(x.out + x.at_a * kElem);
+      x.a.round(a);
+      x.b.round(a + N);
     }
+    x.a.store(x.out + x.at_a * kElem);
+    if (N > 1 || x.at_b != 0) x.b.store(x.out + x.at_b * kElem);
   }
 }
 
-template <class T, bool E4M3, int N>
-void launch_pairs(const RotateParams& p, bool inter, uint32_t wgs, uint32_t lds, hipStream_t s) {
-  if (inter)
-    rotate_append_kernel<T, E4M3, N, true><<<wgs, kThreads, lds, s>>>(p);
+template <class T, bool E4M3, int N, bool INTER>
+void launch_turns(const RotateParams& p, const double* turns, uint32_t wgs, uint32_t lds, hipStream_t s) {
+  const auto filled = [&](auto& t) -> auto& {
+    for (uint32_t i = 0; i < p.half; ++i) t.per_position[i] = turns[i];
+    return t;
+  };
+  const auto go = [&](auto room, auto once) {
+    Turns<decltype(room)::value> t{};
+    rotate_append_kernel<T, E4M3, N, INTER, decltype(room)::value, N != 1 && decltype(once)::value>
+        <<<wgs, kThreads, lds, s>>>(p, filled(t));
+  };
+  const std::integral_constant<int, 64> few;
+  const std::integral_constant<int, 128> many;
+  if (p.half <= 64)
+    p.once ? go(few, std::true_type()) : go(few, std::false_type());
   else
-    rotate_append_kernel<T, E4M3, N, false><<<wgs, kThreads, lds, s>>>(p);
+    p.once ? go(many, std::true_type()) : go(many, std::false_type());
+}
+
+template <class T, bool E4M3, int N>
+void launch_pairs(const RotateParams& p, const double* turns, bool inter, uint32_t wgs, uint32_t lds, hipStream_t s) {
+  if (inter)
+    launch_turns<T, E4M3, N, true>(p, turns, wgs, lds, s);
+  else
+    launch_turns<T, E4M3, N, false>(p, turns, wgs, lds, s);
 }
 
 template <class T, bool E4M3>
-void launch_pieces(const RotateParams& p, bool vec, bool inter, uint32_t wgs, uint32_t lds, hipStream_t s) {
+void launch_pieces(const RotateParams& p, const double* turns, bool vec, bool inter, uint32_t wgs, uint32_t lds,
+                   hipStream_t s) {
   if (vec)
-    launch_pairs<T, E4M3, 16 / Piece<T, 1>::kElem>(p, inter, wgs, lds, s);
+    launch_pairs<T, E4M3, 16 / Piece<T, 1>::kElem>(p, turns, inter, wgs, lds, s);
   else
-    launch_pairs<T, E4M3, 1>(p, inter, wgs, lds, s);
+    launch_pairs<T, E4M3, 1>(p, turns, inter, wgs, lds, s);
 }
 
 struct RotateCall {
@@ -309,44 +340,43 @@ struct RotateCall {
 int launch_rotate(const RotateCall& c, RotateParams& p, const char* who) {
   const uint32_t dim = c.rotary ? c.rotary->dim : 0, n_vec = 16 / dtype_bytes(c.dtype);
   const bool inter = c.rotary && c.rotary->interleaved;
-  // vectors need whole pieces on both sides of a pair, and rows that divide into them
-  const bool vec = c.aligned && dim % (2 * n_vec) == 0 && c.head_dim % n_vec == 0;
+  // vectors need an even number of whole pieces in both parts of a row
+  const bool vec = c.aligned && dim % (2 * n_vec) == 0 && c.head_dim % (2 * n_vec) == 0;
   const uint32_t n = vec ? n_vec : 1;
   p.half = dim / 2;
+  p.dim = c.head_dim;
   p.rot_items = p.half / n;
-  p.row_items = p.rot_items + (c.head_dim - dim) / n;
-  p.v_row_items = c.head_dim / n;
+  p.row_items = p.rot_items + (c.head_dim - dim + 1) / 2 / n;
   p.q_items = c.n_q_heads * p.row_items;
   p.qk_items = p.q_items + c.n_kv_heads * p.row_items;
-  p.items = p.qk_items + c.n_kv_heads * p.v_row_items;
+  p.items = p.qk_items + c.n_kv_heads * p.row_items;
   p.items_magic = division_magic(p.items);
   p.row_magic = division_magic(p.row_items);
-  p.v_row_magic = division_magic(p.v_row_items);
   p.half_magic = division_magic(p.half);
   p.block_magic = division_magic(p.ntpb);
-  if (c.rotary) {
-    p.magnitude = c.rotary->magnitude;
-    for (uint32_t i = 0; i < p.half; ++i) p.turns[i] = c.rotary->turns[i];
-  }
+  if (c.rotary) p.magnitude = c.rotary->magnitude;
+  const double* turns = c.rotary ? c.rotary->turns : nullptr;
   const unsigned __int128 all = static_cast<unsigned __int128>(p.n_tokens) * p.items;
   const unsigned __int128 wgs = (all + kItemsPerWg - 1) / kItemsPerWg;
   if (wgs > 0x7FFFFF00u) return fail(KVT_ERR_INVALID, std::string(who) + ": too many rows for one launch");
   if (wgs == 0) return KVT_OK;
+  p.near = (wgs * kItemsPerWg >> 32) == 0;
+  p.once = all * 2 * n * dtype_bytes(c.dtype) > kCachedInput;
   // tokens that one workgroup's items can belong to
   const uint32_t span = (kItemsPerWg - 2) / p.items + 2;
   const uint32_t lds = span * p.half * static_cast<uint32_t>(sizeof(float2));
   const uint32_t grid = static_cast<uint32_t>(wgs);
   switch (c.dtype) {
     case KVT_DTYPE_BF16:
-      if (c.e4m3) launch_pieces<Bf16, true>(p, vec, inter, grid, lds, c.stream);
-      else launch_pieces<Bf16, false>(p, vec, inter, grid, lds, c.stream);
+      if (c.e4m3) launch_pieces<Bf16, true>(p, turns, vec, inter, grid, lds, c.stream);
+      else launch_pieces<Bf16, false>(p, turns, vec, inter, grid, lds, c.stream);
       break;
     case KVT_DTYPE_F16:
-      if (c.e4m3) launch_pieces<F16, true>(p, vec, inter, grid, lds, c.stream);
-      else launch_pieces<F16, false>(p, vec, inter, grid, lds, c.stream);
+      if (c.e4m3) launch_pieces<F16, true>(p, turns, vec, inter, grid, lds, c.stream);
+      else launch_pieces<F16, false>(p, turns, vec, inter, grid, lds, c.stream);
       break;
     default:
-      launch_pieces<F32, false>(p, vec, inter, grid, lds, c.stream);
+      launch_pieces<F32, false>(p, turns, vec, inter, grid, lds, c.stream);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return hip_fail(e, who);
@@ -391,11 +421,9 @@ int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void
     DeviceGuard g;
     if (int rc = g.enter(device)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (!being_captured(s)) {
-      if (int rc = check_device_span(x, in_span, "kvt_rotary_apply: x")) return rc;
-      if (int rc = check_device_span(out, out_span, "kvt_rotary_apply: out")) return rc;
-      if (int rc = check_device_span(positions, 8 * n_tokens, "kvt_rotary_apply: positions")) return rc;
-    }
+    if (!being_captured(s))
+      if (int rc = check_spans(who, {{x, in_span, "x"}, {out, out_span, "out"}, {positions, 8 * n_tokens, "positions"}}))
+        return rc;
     RotateParams p{};
     p.q = static_cast<const uint8_t*>(x);
     p.q_token = x_token_stride, p.q_head = x_head_stride;
@@ -456,15 +484,10 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
     DeviceGuard g;
     if (int rc = g.enter(cache->device)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (!being_captured(s)) {
-      if (int rc = check_device_span(k, k_span, "kvt_kv_append: k")) return rc;
-      if (int rc = check_device_span(v, v_span, "kvt_kv_append: v")) return rc;
-      if (int rc = check_device_span(q, q_span, "kvt_kv_append: q")) return rc;
-      if (int rc = check_device_span(q_out, qo_span, "kvt_kv_append: q_out")) return rc;
-      if (int rc = check_device_span(slots, 8 * n_tokens, "kvt_kv_append: slots")) return rc;
-      if (rotary)
-        if (int rc = check_device_span(positions, 8 * n_tokens, "kvt_kv_append: positions")) return rc;
-    }
+    if (!being_captured(s))
+      if (int rc = check_spans(who, {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"},
+                                     {slots, 8 * n_tokens, "slots"}, {positions, rotary ? 8 * n_tokens : 0, "positions"}}))
+        return rc;
     RotateParams p{};
     p.q = static_cast<const uint8_t*>(q), p.k = static_cast<const uint8_t*>(k), p.v = static_cast<const uint8_t*>(v);
     p.q_token = q_token_stride, p.q_head = q_head_stride;

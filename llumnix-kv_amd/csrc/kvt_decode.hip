@@ -947,14 +947,11 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     unsigned long long capture = 0;
     if (hipStreamIsCapturing(s, &cap) != hipSuccess) (void)hipGetLastError();
     if (cap == hipStreamCaptureStatusNone) {
-      if (int rc = check_device_span(q, q_span, "kvt_decode_attention: q")) return rc;
-      if (int rc = check_device_span(out, out_span, "kvt_decode_attention: out")) return rc;
-      if (int rc = check_device_span(seq_lens, 4ull * n_seqs, "kvt_decode_attention: seq_lens")) return rc;
-      if (int rc = check_device_span(block_tables, table_blocks ? 4 * ((n_seqs - 1) * table_stride + table_blocks) : 0,
-                                     "kvt_decode_attention: block_tables"))
+      if (int rc = check_spans(
+              who, {{q, q_span, "q"}, {out, out_span, "out"}, {seq_lens, 4ull * n_seqs, "seq_lens"},
+                    {block_tables, table_blocks ? 4 * ((n_seqs - 1) * table_stride + table_blocks) : 0, "block_tables"},
+                    {lse, lse ? 4ull * n_seqs * d->n_heads : 0, "lse"}}))
         return rc;
-      if (lse)
-        if (int rc = check_device_span(lse, 4ull * n_seqs * d->n_heads, "kvt_decode_attention: lse")) return rc;
     } else if (hipStreamGetCaptureInfo(s, &cap, &capture) != hipSuccess || capture == 0) {
       (void)hipGetLastError();
       return fail(KVT_ERR_HIP, "kvt_decode_attention: the stream's capture cannot be told apart");

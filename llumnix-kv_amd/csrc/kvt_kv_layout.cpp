@@ -120,6 +120,14 @@ int check_apart(const Rows& in, uint32_t in_heads, const Rows& out, uint32_t out
                                              " without being the same rows"));
 }
 
+int check_spans(const char* who, std::initializer_list<Span> spans) {
+  static const std::string none;
+  for (const Span& s : spans)
+    if (check_device_span(s.ptr, s.bytes, none) != KVT_OK)
+      return check_device_span(s.ptr, s.bytes, std::string(who) + ": " + s.what);
+  return KVT_OK;
+}
+
 }  // namespace kvt
 
 using namespace kvt;

@@ -3,6 +3,7 @@
 #ifndef KVT_OPS_H_
 #define KVT_OPS_H_
 
+#include <initializer_list>
 #include <string>
 
 #include "kvt_runtime.h"
@@ -40,6 +41,14 @@ int check_rows(const Rows& r, uint64_t n_tokens, uint32_t n_heads, uint64_t row_
 // tensor that interleave without sharing a byte are told apart.
 int check_apart(const Rows& in, uint32_t in_heads, const Rows& out, uint32_t out_heads, uint64_t n_tokens,
                 uint64_t row_bytes, bool in_place, const char* who, const char* what);
+
+// check_device_span() of several buffers; the text of a refusal is only made for one.
+struct Span {
+  const void* ptr;
+  uint64_t bytes;
+  const char* what;
+};
+int check_spans(const char* who, std::initializer_list<Span> spans);
 
 inline bool rows_aligned16(const Rows& r) {
   return ((reinterpret_cast<uintptr_t>(r.ptr) | r.token_stride | r.head_stride) & 15u) == 0;

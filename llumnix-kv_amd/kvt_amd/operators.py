@@ -11,36 +11,43 @@ from . import binding
 from .binding import KvLayoutStruct, RotaryOpts, _quiet_close, check, lib
 
 DTYPES = {"bf16": 0, "f16": 1, "f32": 2, "e4m3": 3}
-_TORCH_NAMES = {"torch.bfloat16": 0, "torch.float16": 1, "torch.float32": 2, "torch.float8_e4m3fn": 3}
-_codes = {}          # torch dtype -> code, filled as they come
 SCALINGS = {"plain": 0, "linear": 1, "bands": 2, "ramp": 3}
+_types = {}          # "int32", "int64" and the codes above -> torch dtype; torch dtype -> code
+
+
+def _torch_types():
+    """Filled by the first call that is given a tensor: this package does without torch."""
+    import torch
+    named = {0: torch.bfloat16, 1: torch.float16, 2: torch.float32}
+    _types.update(named)
+    _types.update({t: code for code, t in named.items()})
+    _types.update(int32=torch.int32, int64=torch.int64)
+    return _types
 
 
 def _code(tensor, name):
-    code = _codes.get(tensor.dtype)
+    code = (_types or _torch_types()).get(tensor.dtype)
     if code is None:
-        code = _codes[tensor.dtype] = _TORCH_NAMES.get(str(tensor.dtype), -1)
-    if code < 0:
         raise ValueError("%s: unsupported type %s" % (name, tensor.dtype))
     return code
 
 
-def _rows(tensor, name, n_tokens, n_heads, dim, code):
+def _rows(tensor, name, shape, code):
     """(pointer, token stride, head stride) in bytes of a [tokens, heads, dim] tensor."""
-    if tuple(tensor.shape) != (n_tokens, n_heads, dim) or _code(tensor, name) != code:
-        raise ValueError("%s: got %s of %s, expected %s" % (name, tuple(tensor.shape), tensor.dtype,
-                                                            (n_tokens, n_heads, dim)))
+    if tensor.shape != shape or tensor.dtype != _types[code]:
+        raise ValueError("%s: got %s of %s, expected %s of %s" % (name, tuple(tensor.shape), tensor.dtype, shape,
+                                                                  _types[code]))
     t, h, e = tensor.stride()
-    if e != 1 and dim > 1:
+    if e != 1 and shape[2] > 1:
         raise ValueError("%s: the elements of a row must lie next to each other" % name)
-    size = tensor.element_size()
+    size = 4 if code == 2 else 2
     return tensor.data_ptr(), t * size, h * size
 
 
-def _index(tensor, name, shape, dtype):
-    """Pointer of a contiguous tensor of one type."""
-    if tuple(tensor.shape) != shape or str(tensor.dtype) != dtype or not tensor.is_contiguous():
-        raise ValueError("%s: expected a contiguous %s tensor of shape %s" % (name, dtype, shape))
+def _index(tensor, name, shape, kind):
+    """Pointer of a contiguous tensor of one type ("int32", "int64" or a code)."""
+    if tensor.shape != shape or tensor.dtype != _types[kind] or not tensor.is_contiguous():
+        raise ValueError("%s: expected a contiguous %s tensor of shape %s" % (name, _types[kind], shape))
     return tensor.data_ptr()
 
 
@@ -93,11 +100,15 @@ class Rotary:
 
     def apply(self, x, positions, out, stream=None):
         """out[t, h] = x[t, h] rotated to positions[t] (int64); out may be x. -> out"""
-        n, heads, dim = x.shape
+        shape = tuple(x.shape)
+        n, heads, dim = shape
         code = _code(x, "x")
-        check(lib().kvt_rotary_apply(self.h, x.get_device(), code, *_rows(x, "x", n, heads, dim, code),
-                                     *_rows(out, "out", n, heads, dim, code),
-                                     _index(positions, "positions", (n,), "torch.int64"), n, heads, dim, stream))
+        x_ptr, x_t, x_h = _rows(x, "x", shape, code)
+        out_ptr, out_t, out_h = _rows(out, "out", shape, code)
+        rc = lib().kvt_rotary_apply(self.h, x.get_device(), code, x_ptr, x_t, x_h, out_ptr, out_t, out_h,
+                                    _index(positions, "positions", (n,), "int64"), n, heads, dim, stream)
+        if rc:
+            check(rc)
         return out
 
     def close(self):
@@ -116,15 +127,22 @@ def kv_append(cache, layer, layout, k, v, slots, rotary=None, positions=None, q=
     (kvt_kv_append)."""
     n, dim = k.shape[0], layout.head_dim
     code = _code(k, "k")
-    q_args, q_heads, out_args = (None, 0, 0), 0, (None, 0, 0)
+    rows = (n, layout.n_kv_heads, dim)
+    k_ptr, k_t, k_h = _rows(k, "k", rows, code)
+    v_ptr, v_t, v_h = _rows(v, "v", rows, code)
+    q_ptr = out_ptr = pos_ptr = None
+    q_t = q_h = q_heads = out_t = out_h = 0
     if q is not None:
         q_heads = q.shape[1]
-        q_args, out_args = _rows(q, "q", n, q_heads, dim, code), _rows(q_out, "q_out", n, q_heads, dim, code)
-    check(lib().kvt_kv_append(cache.h, layer, layout.ref, rotary.h if rotary is not None else None, code,
-                              *_rows(k, "k", n, layout.n_kv_heads, dim, code),
-                              *_rows(v, "v", n, layout.n_kv_heads, dim, code), *q_args, q_heads, *out_args,
-                              None if positions is None else _index(positions, "positions", (n,), "torch.int64"),
-                              _index(slots, "slots", (n,), "torch.int64"), n, k_scale, v_scale, stream))
+        q_ptr, q_t, q_h = _rows(q, "q", (n, q_heads, dim), code)
+        out_ptr, out_t, out_h = _rows(q_out, "q_out", (n, q_heads, dim), code)
+    if positions is not None:
+        pos_ptr = _index(positions, "positions", (n,), "int64")
+    rc = lib().kvt_kv_append(cache.h, layer, layout.ref, rotary.h if rotary is not None else None, code, k_ptr, k_t, k_h,
+                             v_ptr, v_t, v_h, q_ptr, q_t, q_h, q_heads, out_ptr, out_t, out_h, pos_ptr,
+                             _index(slots, "slots", (n,), "int64"), n, k_scale, v_scale, stream)
+    if rc:
+        check(rc)
 
 
 class DecodeAttention:
@@ -142,15 +160,21 @@ class DecodeAttention:
             stream=None):
         """q, out: [seqs, n_q_heads, head_dim]; block_tables: int32 [seqs, blocks]; seq_lens: int32 [seqs];
         lse: float32 [seqs, n_q_heads] or None. max_len: the longest length if known. -> out"""
-        n, dim = q.shape[0], self.layout.head_dim
-        if (block_tables.dim() != 2 or block_tables.shape[0] != n or str(block_tables.dtype) != "torch.int32"
-                or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)):
+        _code(q, "q")
+        n, heads = q.shape[0], self.n_q_heads
+        shape = (n, heads, self.layout.head_dim)
+        columns = block_tables.shape[1] if block_tables.dim() == 2 else -1
+        if columns < 0 or block_tables.shape[0] != n or block_tables.dtype != _types["int32"] or (
+                columns > 1 and block_tables.stride(1) != 1):
             raise ValueError("block_tables: expected int32 [%d, blocks] with contiguous rows" % n)
-        check(lib().kvt_decode_attention(
-            self.h, cache.h, layer, *_rows(q, "q", n, self.n_q_heads, dim, self.code), block_tables.data_ptr(),
-            block_tables.stride(0), block_tables.shape[1], _index(seq_lens, "seq_lens", (n,), "torch.int32"), n,
-            max_len, k_scale, v_scale, *_rows(out, "out", n, self.n_q_heads, dim, self.code),
-            None if lse is None else _index(lse, "lse", (n, self.n_q_heads), "torch.float32"), stream))
+        q_ptr, q_t, q_h = _rows(q, "q", shape, self.code)
+        out_ptr, out_t, out_h = _rows(out, "out", shape, self.code)
+        rc = lib().kvt_decode_attention(
+            self.h, cache.h, layer, q_ptr, q_t, q_h, block_tables.data_ptr(), block_tables.stride(0), columns,
+            _index(seq_lens, "seq_lens", (n,), "int32"), n, max_len, k_scale, v_scale, out_ptr, out_t, out_h,
+            None if lse is None else _index(lse, "lse", (n, heads), 2), stream)
+        if rc:
+            check(rc)
         return out
 
     def release(self, stream=None):

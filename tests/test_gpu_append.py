@@ -168,6 +168,27 @@ def test_append_sizes(n, heads, kv_heads, dim, part, block, inter):
     _append_case("bf16", "e4m3", "hnd", n, heads, kv_heads, dim, part, block, inter=inter, seed=4)
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("kind,dim,part", [("bf16", 128, 128), ("f32", 128, 32), ("f16", 80, 48)])
+def test_long_inputs(kind, dim, part, inter):
+    """More than is expected to be left in a cache, and tokens that no workgroup begins with."""
+    g = _gen(11)
+    r, freq, mag = _rotary(part, inter)
+    n = (140 << 20) // (9 * dim * (4 if kind == "f32" else 2))
+    x = _normal((n, 9, dim), kind, g)
+    pos = torch.randint(0, 100000, (n,), generator=g, device="cuda")
+    out = r.apply(x, pos, torch.empty_like(x))
+    some = torch.cat((torch.arange(64, device="cuda"), torch.randint(0, n, (2000,), generator=g, device="cuda"),
+                      torch.arange(n - 64, n, device="cuda")))
+    exact, scale = oc.rotated(oc.wide(x[some]), pos[some].cpu().numpy(), freq, mag, part, inter)
+    _hold(oc.wide(out[some]), exact, oc.rotation_tolerance(exact, scale, kind))
+    # all of it, by the rows one at a time being what they are together
+    half = torch.empty_like(x)
+    for a in range(0, n, 4096):
+        r.apply(x[a:a + 4096], pos[a:a + 4096], half[a:a + 4096])
+    assert torch.equal(half, out)
+
+
 def test_append_without_rotation_or_queries_copies():
     g = _gen(1)
     cache = torch.zeros((2, 9, 16, 4, 64), device="cuda", dtype=torch.bfloat16)
