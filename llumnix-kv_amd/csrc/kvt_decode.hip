@@ -60,7 +60,7 @@ struct DecodeParams {
   uint32_t visible_max, ntpb, n_blocks, n_seqs, n_heads, head_dim, window;
   uint32_t group, spread, head_rows, rows, teams, slot_heads;
   float scale_log2, cap, cap_in, v_scale;
-  bool q_vec, out_vec;
+  bool q_vec, out_vec, abreast;
 };
 
 struct Bf16 {
@@ -272,14 +272,17 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       for (uint32_t n = threadIdx.x; n < p.n_heads; n += kThreads) p.lse[static_cast<uint64_t>(s) * p.n_heads + n] = -INFINITY;
   }
 
-  // this workgroup's heads; the wavefronts share them out in tiles of 16 (`spread` tiles side by
-  // side) and then the tokens
-  const uint32_t kv_head = member / p.head_rows, head_row = member - kv_head * p.head_rows;
-  const uint32_t head0 = kv_head * p.group + head_row * p.spread * 16u;
-  const uint32_t left = p.group - head_row * p.spread * 16u;
-  const uint32_t n_heads = left < p.spread * 16u ? left : p.spread * 16u;
+  // this workgroup's heads: `spread` bundles of at most 16 that its wavefronts take side by side
+  // before they share out the tokens -- tiles of one KV head's, or (abreast) those of neighbouring KV heads
+  const uint32_t bundle = p.group < 16u ? p.group : 16u;
   const uint32_t tile = wave & (p.spread - 1), turn = wave / p.spread;
-  const uint32_t my_heads = n_heads <= tile * 16u ? 0u : n_heads - tile * 16u < 16u ? n_heads - tile * 16u : 16u;
+  const uint32_t kv_first = p.abreast ? member * p.spread : member / p.head_rows;
+  const uint32_t head_row = p.abreast ? 0u : member - kv_first * p.head_rows;
+  const uint32_t kv_head = kv_first + (p.abreast ? tile : 0u);
+  const uint32_t head0 = kv_first * p.group + head_row * p.spread * 16u;
+  const uint32_t left = p.abreast ? p.spread * p.group : p.group - head_row * p.spread * 16u;
+  const uint32_t n_heads = left < p.spread * bundle ? left : p.spread * bundle;
+  const uint32_t my_heads = n_heads <= tile * bundle ? 0u : n_heads - tile * bundle < bundle ? n_heads - tile * bundle : bundle;
   const uint32_t step = kStep / p.spread;
 
   const uint8_t* kbase = p.base + kv_head * p.head_stride;
@@ -334,7 +337,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       const uint32_t d = E4M3 ? (c / 2) * 64u + kg * 16u + (c & 1) * 8u : c * 32u + kg * 8u;
       u32x4 v = {0, 0, 0, 0};
       if (col < my_heads && (EXACT || d < dim)) {
-        const uint8_t* a = p.q + seq * p.q_token + (head0 + tile * 16u + col) * p.q_head + d * 2u;
+        const uint8_t* a = p.q + seq * p.q_token + (head0 + tile * bundle + col) * p.q_head + d * 2u;
         if (p.q_vec) {
           v = *reinterpret_cast<const u32x4*>(a);
         } else {
@@ -572,12 +575,11 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     constexpr uint32_t kRow = D + 4;
     Stat* stats = reinterpret_cast<Stat*>(lds);   // [wave][16]
     float* part = lds + kWaves * 16 * 2;
-    const uint32_t tile_heads = p.group < 16u ? p.group : 16u;
     sum = over_tokens_sum(sum);
     if (sum == 0.0f && any) sum = -1.0f;
     if (kg == 0) stats[wave * 16 + col] = Stat{top, sum};
     if (col < my_heads) {
-      float* row = part + (wave * tile_heads + col) * kRow;
+      float* row = part + (wave * bundle + col) * kRow;
 #pragma unroll
       for (int h = 0; h < NP; ++h)
 #pragma unroll
@@ -611,7 +613,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     };
     for (uint32_t n = threadIdx.x; n < work; n += kThreads) {
       const uint32_t head = n / quads, d = (n - head * quads) * 4;
-      const uint32_t t = head / 16u, h = head - t * 16u;
+      const uint32_t t = head / bundle, h = head - t * bundle;
       float m = -INFINITY, l = 0.0f;
       bool inf = false;
       f32x4 o = {0, 0, 0, 0};
@@ -622,7 +624,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
         inf = inf || s.sum < 0.0f;
         if (f != 0.0f) {
           l += f * s.sum;
-          o += f * *reinterpret_cast<const f32x4*>(part + (w * tile_heads + h) * kRow + d);
+          o += f * *reinterpret_cast<const f32x4*>(part + (w * bundle + h) * kRow + d);
         }
       }
       if (whole) {
@@ -746,6 +748,14 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
   }
 }
 
+// Where the rows of neighbouring KV heads are neighbours in memory and short, a workgroup takes two
+// of them side by side, so that it reads 512 bytes in a row instead of 256 (twice the sums to join,
+// hence only where every workgroup has this many units). One / two heads, microseconds, 8 KV heads of
+// 128 bf16 in [.., h, d] rows: 64 sequences of 1k-8k 196.6 / 182.7, 16 of them 49.2 / 45.8, 12 38.9 /
+// 39.9, 8 31.9 / 36.6; rows of 512 bytes (dim 256) 310 / 316; 2 KV heads (e4m3) 74.5 / 75.7; pages that
+// keep a head's rows together 169.8 / 171.2.
+constexpr uint32_t kAbreastUnits = 8;
+
 struct Launch {
   dim3 grid;
   uint32_t lds;
@@ -808,8 +818,9 @@ struct kvt_decode {
   std::vector<Owner> owners;
 
   uint32_t n_wgs = 0, teams = 0;
-  uint64_t ml_at() const { return round_up(n_wgs * 2ull * slot_heads * layout.head_dim * 4, 256); }
-  uint64_t counters_at() const { return round_up(ml_at() + n_wgs * 2ull * slot_heads * 8, 256); }
+  bool pairs = false;   // neighbouring KV heads may be taken side by side
+  uint64_t ml_at() const { return round_up(n_wgs * 2ull * slot_heads * (pairs ? 2 : 1) * layout.head_dim * 4, 256); }
+  uint64_t counters_at() const { return round_up(ml_at() + n_wgs * 2ull * slot_heads * (pairs ? 2 : 1) * 8, 256); }
 
   int workspace(hipStream_t s, unsigned long long capture, uint8_t** out) {
     const std::thread::id me = s == hipStreamPerThread ? std::this_thread::get_id() : std::thread::id();
@@ -871,6 +882,9 @@ int kvt_decode_create(int device, const kvt_kv_layout* layout, uint32_t dtype, u
     d->rows = layout->n_kv_heads * d->head_rows;
     d->teams = std::max(1u, device_cu_count(device) * per_cu(layout->head_dim) / d->rows);
     d->n_wgs = d->teams * d->rows;
+    const uint32_t row = layout->head_dim * dtype_bytes(layout->dtype);
+    d->pairs = d->group <= 16 && layout->n_kv_heads >= 4 && layout->n_kv_heads % 2 == 0 && row <= 256 &&
+               layout->head_stride == row;
     const uint64_t counters = d->n_wgs;
     d->ws_bytes = round_up(d->counters_at() + counters * 4, 256);
     d->owners.resize(n_workspaces);
@@ -981,7 +995,14 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     p.rows = d->rows;
     uint64_t longest = max_len == 0 || max_len > p.visible_max ? p.visible_max : max_len;
     const uint64_t units = (longest + kStep - 1) / kStep * n_seqs;
-    p.teams = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(d->teams, units)));
+    uint32_t teams = d->teams;
+    if (d->pairs && units >= kAbreastUnits * d->n_wgs / (d->rows / 2)) {
+      p.abreast = true;
+      p.spread = 2, p.head_rows = 1, p.slot_heads = 2 * d->group;
+      p.rows = d->rows / 2;
+      teams = d->n_wgs / p.rows;
+    }
+    p.teams = static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(teams, units)));
     const uint32_t wgs = p.teams * p.rows;
     {
       uint8_t* ws = nullptr;

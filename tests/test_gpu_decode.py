@@ -286,6 +286,20 @@ def test_uneven_sequences_in_many_shares():
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("kind,cache_kind,layout,heads,kv_heads,dim,block", [
+    ("bf16", "bf16", "flash", 8, 4, 128, 16), ("f16", "f16", "ragged", 20, 4, 80, 5), ("bf16", "e4m3", "pages", 96, 6, 256, 16),
+    ("bf16", "bf16", "flash", 4, 4, 64, 16)])
+def test_batches_large_enough_to_take_two_heads_side_by_side(kind, cache_kind, layout, heads, kv_heads, dim, block):
+    rng = np.random.default_rng(22)
+    lens = [int(n) for n in rng.integers(0, 400, 200)] + [0, 1, 2500]
+    c = Case(kind, cache_kind, layout, lens, heads, kv_heads, dim, block, seed=22)
+    op, exact = c.operator(), c.exact()
+    many = c.check(op, exact, max_len=100000)      # as many units as make it worth it, says the caller
+    c.check(op, exact, max_len=1)
+    again = c.check(op, exact, max_len=100000)
+    assert torch.equal(many[0], again[0]) and torch.equal(many[1], again[1])
+
+
 def test_pages_of_a_cache_beyond_32_bits_that_end_inside_a_tile():
     """Offsets that need 64 bits and block sizes that are no multiple of 16: a cache of 5 GiB."""
     block, kv, dim = 5, 1, 256
