@@ -935,7 +935,7 @@ int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void
  * slots[t] outside [0, n_blocks * ntpb) -- padding, -1 -- leaves the cache alone (the query row
  * is rotated all the same); every other row of the cache keeps its bytes. Two tokens of one call
  * with the same slot leave an unspecified mixture of their rows in it. Inputs may be slices of a
- * wider tensor (strides as in kvt_rotary_apply). */
+ * wider tensor (strides as in kvt_rotary_apply); they lie outside the cache's tensor. */
 int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* layout,
                   const kvt_rotary* rotary, uint32_t dtype, const void* k, uint64_t k_token_stride,
                   uint64_t k_head_stride, const void* v, uint64_t v_token_stride,
@@ -956,8 +956,9 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
  * [0, n_blocks). A sequence that sees no token (a padding row: length 0 or negative) gets zeros and
  * an lse of minus infinity. Rows of the cache that are not seen may hold anything, NaN included.
  * Scores, weights, sums and the maximum are held in 32 bits, the weights take part in the product
- * with V as two 16-bit values each; every output is rounded once. Results do not depend on the
- * order in which workgroups run.
+ * with V as two 16-bit values each; every output is rounded once. The same call gives the same
+ * bits each time; the other sequences of a batch and max_len move a sequence's result within the
+ * rounding of its 32-bit sums, since they decide where it is split.
  *
  * An operator holds the layout, the heads and workspaces for sums of sequences that are split over
  * several workgroups. It is meant to be kept: one serves all layers of a model and any number of

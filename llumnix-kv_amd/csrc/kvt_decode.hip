@@ -192,8 +192,9 @@ __device__ __forceinline__ uint32_t units_of(const DecodeParams& p, int32_t raw)
 struct Stat {
   float max, sum;
 };
+// (the maximum passes over NaN: a part of nothing but NaN has no maximum, and a NaN sum)
 __device__ __forceinline__ float weight_of(const Stat& s, float top) {
-  return s.max == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s.max - top);
+  return s.max != -INFINITY ? __builtin_amdgcn_exp2f(s.max - top) : s.sum != s.sum ? s.sum : 0.0f;
 }
 
 enum { kWhole, kNear, kFar };

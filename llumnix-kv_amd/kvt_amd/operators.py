@@ -133,6 +133,8 @@ def kv_append(cache, layer, layout, k, v, slots, rotary=None, positions=None, q=
     q_ptr = out_ptr = pos_ptr = None
     q_t = q_h = q_heads = out_t = out_h = 0
     if q is not None:
+        if q_out is None:
+            raise ValueError("q without q_out")
         q_heads = q.shape[1]
         q_ptr, q_t, q_h = _rows(q, "q", (n, q_heads, dim), code)
         out_ptr, out_t, out_h = _rows(q_out, "q_out", (n, q_heads, dim), code)

@@ -222,6 +222,23 @@ def test_strided_and_unaligned_queries_and_outputs():
     c.check(op, exact)
 
 
+@pytest.mark.parametrize("max_len", [0, 1])
+@pytest.mark.parametrize("where", ["alone", "all", "a whole part", "beside minus infinity"])
+def test_scores_that_are_nan_and_nothing_else(where, max_len):
+    c = Case("bf16", "bf16", "flash", [1 if where == "alone" else 700, 33], 4, 1, 64, 16, seed=23)
+    k = oc.kv_views("flash", c.cache)[0].view(torch.bfloat16)
+    n = c.lens[0]
+    at = {"alone": range(n), "all": range(n), "a whole part": range(512, 640), "beside minus infinity": range(n)}[where]
+    c.q[0] = c.q[0].abs() + 0.5
+    for t in at:
+        k[int(c.tables[0, t // 16]), t % 16][0, 3] = float("-inf" if where.startswith("beside") and t != 300 else "nan")
+    out, lse = c.buffers()
+    c.operator().run(c.handle, 0, c.q, c.d_tables, c.d_lens, out, lse=lse, max_len=max_len)
+    assert np.isnan(oc.wide(out)[0]).all() and np.isnan(oc.wide(lse)[0]).all()
+    exact = oc.decode_exact(oc.wide(c.q)[1:], *c.plain, c.tables[1:], [33], 16, 64 ** -0.5)
+    hold(out[1:], lse[1:], exact, "bf16")
+
+
 def test_infinities_and_nan_that_are_seen_follow_the_formula():
     c = Case("bf16", "bf16", "flash", [200, 200, 200, 200], 4, 1, 64, 16, seed=10)
     k, v = (x.view(torch.bfloat16) for x in oc.kv_views("flash", c.cache))
@@ -249,6 +266,40 @@ def test_infinities_and_nan_that_are_seen_follow_the_formula():
     plain[0][b, r, 0, 5] = -1e30
     exact = oc.decode_exact(oc.wide(c.q)[1:2], *plain, c.tables[1:2], [200], 16, 64 ** -0.5)
     hold(out[1:2], lse[1:2], exact, "bf16")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_every_8_bit_value_is_itself(kind):
+    """One token: the output is its row of V, times the scale; NaN included. As keys: scores that are
+    the value times a query of one."""
+    cache = torch.zeros((1, 1, 2, 1, 256), device="cuda", dtype=torch.uint8)
+    cache[0, 0, 1, 0] = torch.arange(256, device="cuda").to(torch.uint8)
+    handle = kvt_amd.Cache(0, [[cache]], [512])
+    lay = kvt_amd.KvLayout(kvt_amd.SHAPE_RAGGED_FLASH, "e4m3", 1, 1, 1, 256)
+    op = kvt_amd.DecodeAttention(0, lay, kind, 1, max_seqs=1)
+    q, out = (torch.zeros((1, 1, 256), device="cuda", dtype=oc.torch_type(kind)) for _ in range(2))
+    table, one = (torch.full(s, v, device="cuda", dtype=torch.int32) for s, v in (((1, 1), 0), ((1,), 1)))
+    op.run(handle, 0, q, table, one, out)
+    want = oc.wide(cache[0, 0, 1, 0].view(torch.float8_e4m3fn))
+    assert np.array_equal(oc.wide(out)[0, 0], want, equal_nan=True)
+    op.run(handle, 0, q, table, one, out, v_scale=0.5)
+    assert np.array_equal(oc.wide(out)[0, 0], want * 0.5, equal_nan=True)
+    # 256 tokens of one dim that counts: lse of each alone is the score
+    keys = torch.zeros((256, 1, 2, 1, 16), device="cuda", dtype=torch.uint8)
+    keys[:, 0, 0, 0, 3] = torch.arange(256, device="cuda").to(torch.uint8)
+    handle = kvt_amd.Cache(0, [[keys]], [keys.numel()])
+    lay = kvt_amd.KvLayout(kvt_amd.SHAPE_RAGGED_FLASH, "e4m3", 256, 1, 1, 16)
+    op = kvt_amd.DecodeAttention(0, lay, kind, 1, max_seqs=256, softmax_scale=1.0)
+    q = torch.zeros((256, 1, 16), device="cuda", dtype=oc.torch_type(kind))
+    q[:, 0, 3] = 1
+    lse = torch.empty((256, 1), device="cuda")
+    op.run(handle, 0, q, torch.arange(256, device="cuda", dtype=torch.int32)[:, None],
+           torch.ones(256, device="cuda", dtype=torch.int32), torch.empty_like(q), lse=lse)
+    got = oc.wide(lse)[:, 0]
+    # (log2 e in, ln 2 out: two roundings of 32 bits each)
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    held = ~np.isnan(want)
+    assert (np.abs(got - want)[held] <= 4 * 2.0 ** -24 * np.abs(want)[held] + 2.0 ** -30).all()
 
 
 def test_long_sequences_split_over_the_device():

@@ -181,3 +181,54 @@ def test_layouts_whose_rows_meet_are_refused(strides):
     lay = kvt_amd.KvLayout(None, "bf16", 64, 16, 8, 128, strides=strides)
     assert _append(lay, kvt_amd.Rotary(128)) == ERR_INVALID
     assert b"null cache" not in kvt_amd.lib().kvt_last_error()
+
+
+def test_decode_create_refuses_on_the_host():
+    lay = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128)
+    lay8 = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "e4m3", 64, 16, 8, 128)
+    new = kvt_amd.DecodeAttention
+    _refused(ERR_UNSUPPORTED, new, 0, lay, "f16", 32, 4)             # not the cache's type
+    _refused(ERR_UNSUPPORTED, new, 0, lay8, "f32", 32, 4)
+    _refused(ERR_UNSUPPORTED, new, 0, lay8, "e4m3", 32, 4)
+    for heads in (0, 7, 12, 8 * 65536):
+        _refused(ERR_INVALID, new, 0, lay, "bf16", heads, 4)
+    for kw in (dict(max_seqs=0), dict(max_seqs=65536), dict(workspaces=0), dict(workspaces=1025),
+               dict(logit_cap=-1.0), dict(logit_cap=math.inf), dict(softmax_scale=math.nan), dict(softmax_scale=math.inf)):
+        _refused(ERR_INVALID, new, 0, lay, "bf16", 32, **dict(dict(max_seqs=4), **kw))
+    bad = kvt_amd.KvLayout(None, "bf16", 64, 16, 8, 128, strides=(65536, 1 << 22, 255, 4096))
+    _refused(ERR_INVALID, new, 0, bad, "bf16", 32, 4)
+    lib = kvt_amd.lib()
+    assert lib.kvt_decode_create(0, lay.ref, 0, 32, 0.0, 0.0, 0, 4, 1, None) == ERR_INVALID
+    assert lib.kvt_decode_create(0, None, 0, 32, 0.0, 0.0, 0, 4, 1, C.byref(C.c_void_p())) == ERR_INVALID
+    assert lib.kvt_decode_attention(None, None, 0, P, 0, 0, P, 0, 1, P, 1, 0, 1.0, 1.0, P, 0, 0, None, None) == ERR_INVALID
+    assert lib.kvt_decode_release(None, None) == ERR_INVALID
+    lib.kvt_decode_destroy(None)
+
+
+@pytest.mark.skipif(kvt_amd.device_count() > 0, reason="this check is for machines without a GPU")
+def test_decode_create_needs_a_device():
+    lay = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128)
+    _refused(ctypes_defs.ERR_NO_DEVICE, kvt_amd.DecodeAttention, 0, lay, "bf16", 32, 4)
+
+
+def test_the_binding_checks_sizes_and_types_before_the_library():
+    import torch
+    lay = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 2, 64)
+    r = kvt_amd.Rotary(64)
+    rows, slots = torch.zeros((3, 2, 64), dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+
+    class NoCache:
+        h = None
+
+    ok = dict(k=rows, v=rows, slots=slots)
+    for bad in (dict(v=rows[:2]), dict(v=rows.half()), dict(slots=slots.int()), dict(slots=slots[:2]),
+                dict(k=rows.double()), dict(v=rows[..., ::2]), dict(k=rows[..., :32], v=rows[..., :32]),
+                dict(q=rows), dict(q=rows, q_out=rows.float()), dict(rotary=r, positions=slots.float())):
+        with pytest.raises(ValueError):
+            kvt_amd.kv_append(NoCache, 0, lay, **dict(ok, **bad))
+    with pytest.raises(ValueError):
+        r.apply(rows, slots, rows[:2])
+    with pytest.raises(ValueError):
+        r.apply(rows, slots[:1], rows)
+    with pytest.raises(ValueError):
+        r.apply(rows.transpose(1, 2), slots, rows.transpose(1, 2))
