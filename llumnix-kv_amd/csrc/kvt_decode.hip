@@ -18,7 +18,10 @@
 // them once costs as much error as the output's rounding does, the second product costs a few
 // matrix instructions in a kernel that is bound by HBM. Both values are positive (the rest at
 // least the smallest positive number), so that an infinity in V times a weight is that infinity,
-// as in the formula, and not the difference of two.
+// as in the formula, and not the difference of two. For f16 the weights are taken times 2^15, which
+// makes its smallest positive number 2^-39 of the largest weight: 2^-24 of it, for each of the many
+// small weights of a long sequence in which one token stands out, would add up to more than the
+// output's own rounding.
 //
 // An 8-bit cache is widened on load: every e4m3 value is a bf16 and an f16 value.
 #include <hip/hip_runtime.h>
@@ -73,11 +76,12 @@ struct Bf16 {
   static __device__ __forceinline__ uint32_t widen(uint32_t e4m3) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(e4m3, 1.0f, HIGH));
   }
-  // two values cut off to this type, and the smallest positive rest worth adding (see Weights)
+  // two values cut off to this type, its smallest positive number worth adding, and what the
+  // largest weight is in the product with V
   static __device__ __forceinline__ uint32_t cut(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
   }
-  static constexpr float kLeast = 0x1p-126f;
+  static constexpr float kLeast = 0x1p-126f, kTop = 1.0f;
 };
 struct F16 {
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
@@ -92,7 +96,7 @@ struct F16 {
   static __device__ __forceinline__ uint32_t cut(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
   }
-  static constexpr float kLeast = 0x1p-24f;
+  static constexpr float kLeast = 0x1p-24f, kTop = 0x1p15f;
 };
 
 // N pieces of 16 bytes from LDS, once all but the newest `NEWER` vector memory operations are done:
@@ -516,8 +520,9 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int s = i >> 1, r = 2 * (i & 1);
-        const float a = __builtin_amdgcn_exp2f(sc[s][r] - ref), b = __builtin_amdgcn_exp2f(sc[s][r + 1] - ref);
+        float a = __builtin_amdgcn_exp2f(sc[s][r] - ref), b = __builtin_amdgcn_exp2f(sc[s][r + 1] - ref);
         sum += a + b;
+        a *= T::kTop, b *= T::kTop;
         const uint32_t hi = T::cut(a, b);
         const f32x2 kept = __builtin_convertvector(__builtin_bit_cast(typename T::x2, hi), f32x2);
         const f32x2 rest = {fmaxf(a - kept.x, T::kLeast), fmaxf(b - kept.y, T::kLeast)};
@@ -596,7 +601,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     const uint32_t quads = dim / 4, work = n_heads * quads;
     const bool whole = n_units == units;
     const auto finish = [&](uint32_t head, uint32_t d, f32x4 o, float m, float l, bool nothing_but_inf) {
-      const float inv = l == 0.0f ? (nothing_but_inf ? NAN : 0.0f) : p.v_scale / l;
+      const float inv = l == 0.0f ? (nothing_but_inf ? NAN : 0.0f) : p.v_scale / T::kTop / l;
       uint8_t* a = p.out + seq * p.out_token + (head0 + head) * p.out_head + d * 2u;
       o *= inv;
       const f32x2 lo = {o.x, o.y}, hi = {o.z, o.w};

@@ -104,14 +104,14 @@ def decode_tolerance(out, lse, measure, kind):
     16-bit values are exact); the weights of a softmax by twice that, relative, and 4 roundings of
     the exponential. Sums over n tokens: n roundings of 2^-24 of the sum of p |v|. A weight in two
     16-bit values, cut off (a step, 2^-7 for bf16 and 2^-10 for f16) and the rest rounded (half a
-    step): 2^-15 or 2^-21 of it; the rest is at least the smallest positive number, for f16 2^-24 of
-    every |v|, and rounded by half of that. Joining parts and dividing: 8 more. Then the output's own rounding."""
+    step): 2^-15 or 2^-21 of it; the rest is at least the smallest positive number, for f16 (2^-24, of
+    weights times 2^15) 2^-39 of every |v|, and rounded by half of that. Joining parts and dividing: 8 more. Then the output's own rounding."""
     mass, size, count, most = measure
     dim = out.shape[-1]
     score = (dim + 8) * 2.0 ** -24 * size
     split = 2.0 ** -15 if kind == "bf16" else 2.0 ** -21
     rel = 2 * score + (12 + count) * 2.0 ** -24 + split
-    tol = rel[..., None] * mass + (0 if kind == "bf16" else 1.5 * 2.0 ** -24 * (count * most)[..., None])
+    tol = rel[..., None] * mass + (0 if kind == "bf16" else 1.5 * 2.0 ** -39 * (count * most)[..., None])
     half, floor = HALF_STEP[kind]
     seen = np.isfinite(lse)
     return (half * (np.abs(out) + tol) + floor + tol,

@@ -302,6 +302,28 @@ def test_every_8_bit_value_is_itself(kind):
     assert (np.abs(got - want)[held] <= 4 * 2.0 ** -24 * np.abs(want)[held] + 2.0 ** -30).all()
 
 
+@pytest.mark.parametrize("kind,cache_kind", [("bf16", "bf16"), ("f16", "f16"), ("f16", "e4m3")])
+@pytest.mark.parametrize("gap", [4.0, 11.0, 16.0, 20.0, 28.0])
+def test_one_token_that_stands_out_of_many(kind, cache_kind, gap):
+    """Weights of exp(-gap) against 1, thousands of them: what each is rounded by must not add up."""
+    n = 30011
+    c = Case(kind, cache_kind, "flash", [n], 4, 1, 64, 16, seed=24)
+    where = c.tables[0, np.arange(n) // 16], np.arange(n) % 16
+    for view, plain, value in zip(oc.kv_views("flash", c.cache), c.plain, (0.0, 10.0)):
+        row = torch.full((64,), value).to(c.cache_type)
+        view[torch.from_numpy(where[0]).cuda(), torch.from_numpy(where[1]).cuda()] = row.view(view.dtype).cuda()
+        plain[where] = value
+    one = int(c.tables[0, 700]), 3
+    for view, plain, value in zip(oc.kv_views("flash", c.cache), c.plain, (4.0, 0.0)):
+        view[one] = torch.full((1, 64), value).to(c.cache_type).view(view.dtype).cuda()
+        plain[one] = value
+    c.q.fill_(0)
+    c.q[:, :, 5] = gap / 4                                   # (exact in every type)
+    exact, op = c.exact(scale=1.0), c.operator(softmax_scale=1.0)
+    for max_len in (0, 1):
+        c.check(op, exact, max_len=max_len)
+
+
 def test_long_sequences_split_over_the_device():
     for kind, cache_kind, layout, n, heads, kv, dim, block in (
             ("bf16", "bf16", "flash", 20011, 8, 2, 128, 16), ("f16", "e4m3", "hnd", 33333, 4, 1, 64, 64),
