@@ -935,7 +935,7 @@ int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void
  * slots[t] outside [0, n_blocks * ntpb) -- padding, -1 -- leaves the cache alone (the query row
  * is rotated all the same); every other row of the cache keeps its bytes. Two tokens of one call
  * with the same slot leave an unspecified mixture of their rows in it. Inputs may be slices of a
- * wider tensor (strides as in kvt_rotary_apply); they lie outside the cache's tensor. */
+ * wider tensor (strides as in kvt_rotary_apply); they, and q_out, lie outside the cache's tensor. */
 int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* layout,
                   const kvt_rotary* rotary, uint32_t dtype, const void* k, uint64_t k_token_stride,
                   uint64_t k_head_stride, const void* v, uint64_t v_token_stride,
@@ -982,7 +982,7 @@ void kvt_decode_destroy(kvt_decode* d);
 /* Gives back what `stream` holds: its eager workspace and those of the captures made on it. Call
  * it when the stream's launches have run and its graphs are gone (before the stream is destroyed). */
 int kvt_decode_release(kvt_decode* d, void* stream);
-/* q, out: rows as in kvt_rotary_apply (out may not share bytes with q). block_tables: int32, row b
+/* q, out: rows as in kvt_rotary_apply (q, out, lse and, for what is written, the cache's tensor share no bytes). block_tables: int32, row b
  * at b * table_stride entries; seq_lens: int32. max_len: the longest length of the batch as far as
  * the host knows it (0: the whole table); it decides how far sequences are split, never the result. */
 int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, const void* q,

@@ -481,6 +481,9 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
     uint8_t* base = nullptr;
     if (int rc = check_cache_layer(cache, layer, layout, extent, who, &base)) return rc;
     if (n_tokens == 0) return KVT_OK;
+    if (int rc = check_distinct(who, {base, extent, "the cache's tensor"},
+                                {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"}}))
+      return rc;
     DeviceGuard g;
     if (int rc = g.enter(cache->device)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -959,6 +959,9 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     if (!seq_lens || (reinterpret_cast<uintptr_t>(seq_lens) & 3u) || (reinterpret_cast<uintptr_t>(lse) & 3u) ||
         (table_blocks != 0 && (!block_tables || (reinterpret_cast<uintptr_t>(block_tables) & 3u))))
       return fail(KVT_ERR_INVALID, "kvt_decode_attention: tables, lengths or lse are null or not aligned");
+    const Span outs{out, out_span, "out"}, lses{lse, lse ? 4ull * n_seqs * d->n_heads : 0, "lse"};
+    if (int rc = check_distinct(who, {base, d->extent, "the cache's tensor"}, {outs, lses})) return rc;
+    if (int rc = check_distinct(who, lses, {outs, {q, q_span, "q"}})) return rc;
     if (table_stride > (1ull << 40)) return fail(KVT_ERR_INVALID, "kvt_decode_attention: table_stride out of range");
     DeviceGuard g;
     if (int rc = g.enter(d->device)) return rc;
@@ -968,9 +971,9 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     if (hipStreamIsCapturing(s, &cap) != hipSuccess) (void)hipGetLastError();
     if (cap == hipStreamCaptureStatusNone) {
       if (int rc = check_spans(
-              who, {{q, q_span, "q"}, {out, out_span, "out"}, {seq_lens, 4ull * n_seqs, "seq_lens"},
+              who, {{q, q_span, "q"}, outs, {seq_lens, 4ull * n_seqs, "seq_lens"},
                     {block_tables, table_blocks ? 4 * ((n_seqs - 1) * table_stride + table_blocks) : 0, "block_tables"},
-                    {lse, lse ? 4ull * n_seqs * d->n_heads : 0, "lse"}}))
+                    lses}))
         return rc;
     } else if (hipStreamGetCaptureInfo(s, &cap, &capture) != hipSuccess || capture == 0) {
       (void)hipGetLastError();

@@ -120,6 +120,16 @@ int check_apart(const Rows& in, uint32_t in_heads, const Rows& out, uint32_t out
                                              " without being the same rows"));
 }
 
+int check_distinct(const char* who, const Span& a, std::initializer_list<Span> others) {
+  const uint64_t a0 = reinterpret_cast<uintptr_t>(a.ptr);
+  for (const Span& b : others) {
+    const uint64_t b0 = reinterpret_cast<uintptr_t>(b.ptr);
+    if (a.bytes != 0 && b.bytes != 0 && a0 < b0 + b.bytes && b0 < a0 + a.bytes)
+      return fail(KVT_ERR_INVALID, text(who, std::string(a.what) + " shares bytes with " + b.what));
+  }
+  return KVT_OK;
+}
+
 int check_spans(const char* who, std::initializer_list<Span> spans) {
   static const std::string none;
   for (const Span& s : spans)

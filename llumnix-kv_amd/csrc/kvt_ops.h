@@ -49,6 +49,8 @@ struct Span {
   const char* what;
 };
 int check_spans(const char* who, std::initializer_list<Span> spans);
+// Refuses a buffer that reaches into one of the others.
+int check_distinct(const char* who, const Span& a, std::initializer_list<Span> others);
 
 inline bool rows_aligned16(const Rows& r) {
   return ((reinterpret_cast<uintptr_t>(r.ptr) | r.token_stride | r.head_stride) & 15u) == 0;

@@ -254,6 +254,14 @@ def test_append_refusals_that_need_a_cache():
         host = torch.ones((3, 2, 64), dtype=torch.bfloat16)
         kvt_amd.kv_append(handle, 0, lay, host, host, slots)
     assert e.value.code == ERR_INVALID
+    inside = cache.flatten()[-3 * 2 * 64:].view(3, 2, 64)
+    r, pos = kvt_amd.Rotary(64), torch.zeros(3, device="cuda", dtype=torch.int64)
+    for rotated in (dict(k=inside, v=rows), dict(k=rows, v=inside),
+                    dict(k=rows, v=rows, q=rows.clone(), q_out=inside, rotary=r, positions=pos),
+                    dict(k=rows, v=rows, q=inside, q_out=rows.clone(), rotary=r, positions=pos)):
+        with pytest.raises(kvt_amd.KvtError) as e:       # rows of the cache itself
+            kvt_amd.kv_append(handle, 0, lay, slots=slots, **rotated)
+        assert e.value.code == ERR_INVALID and "the cache's tensor" in str(e.value)
     with pytest.raises(ValueError):
         kvt_amd.kv_append(handle, 0, lay, rows, rows[:2], slots)
     with pytest.raises(ValueError):

@@ -523,6 +523,11 @@ def test_refusals():
     refused(ERR_INVALID, lambda: op.run(c.handle, 0, c.q, c.d_tables, c.d_lens, out[:1].expand(2, 4, 64)))
     small = kvt_amd.Cache(0, [[c.cache]], [c.cache.numel()])
     refused(ERR_OUT_OF_RANGE, lambda: op.run(small, 0, c.q, c.d_tables, c.d_lens, out))
+    refused(ERR_INVALID, lambda: op.run(c.handle, 0, c.q, c.d_tables, c.d_lens,
+                                        c.cache.view(torch.bfloat16).flatten()[-512:].view(2, 4, 64)))
+    for over in (out, c.q, c.cache):
+        floats = over.view(torch.float32).flatten()[:8].view(2, 4)
+        refused(ERR_INVALID, lambda: op.run(c.handle, 0, c.q, c.d_tables, c.d_lens, out, lse=floats))
     for bad in (dict(q=c.q[:, :3]), dict(q=c.q.half()), dict(block_tables=c.d_tables.long()),
                 dict(seq_lens=c.d_lens[:1]), dict(lse=lse.half())):
         args = dict(q=c.q, block_tables=c.d_tables, seq_lens=c.d_lens, out=out)
