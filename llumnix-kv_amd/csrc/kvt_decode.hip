@@ -24,6 +24,32 @@
 // output's own rounding.
 //
 // An 8-bit cache is widened on load: every e4m3 value is a bf16 and an f16 value.
+//
+// Bound by HBM once a launch has some ten microseconds of rows to read: 4 operations per cached
+// element and query head, 16 to 64 a byte, against the 180 a byte at which the matrix units would take
+// over. What the rest of this file is about is keeping enough reads in flight from every CU, and
+// leaving nothing but reads between the first row and the last:
+//   shares   the units of 128 tokens of all sequences, one list, cut into as many equal shares as
+//            workgroups are resident, wherever that falls: no workgroup waits for a longer one, no second
+//            wave of workgroups starts (one and a half to four times as many: 131071 tokens 94 -> 100-120
+//            us, 128 x 4096 of 256 160 -> 174-187). Every wavefront finds its share itself from the
+//            lengths (a scan, 1 us), so lengths stay on the device and a captured launch serves any.
+//   joins    a row that is split is joined by whichever workgroup is last, in the parts' order (the same
+//            bits each time). Parts are written through and read past the L2s (sc1) and counted by one
+//            relaxed atomic: a device-wide fence per workgroup, which writes back and drops whole L2s,
+//            took 543 us where this takes 292 (64 x 1k-8k tokens, the form before K went through LDS).
+//   K        by whole rows through LDS, without passing registers: reading 64-byte pieces of 16 rows
+//            straight into the matrix operand took 225 us (195), 178 (160) for 256 f16. V stays in
+//            registers, transposed by byte permutes; through LDS as well it gains nothing (196).
+//   ahead    the next tile's rows are asked for before this one's are used up, the block ids of the one
+//            behind before that. Loads are non-temporal: plain ones 230 us (219), 134 (118) for one
+//            long sequence (both before K went through LDS).
+// Microseconds, and TB/s of the bytes a launch cannot do without, where a 1 GiB copy reaches 6.6: 64
+// sequences of 1k-8k tokens, 32 heads on 8 of 128 bf16, 182 (6.4); 128 of 4096, 16 on 2 of 256 f16, 160 (6.7);
+// one of 131071, 64 on 8 of 128 bf16 HND, 93 (5.8: 4 us to the first rows, 10 for the join of 64 parts);
+// 96 of 1-16384, 16 on 2 of 128 e4m3, 75 (5.2: the same, and the matrix units 20 % busy); one of 512, 9.1
+// (one round trip after another: lengths 1, table 2, rows 1.3, the wavefronts' join 0.4, parts out 1.3, the
+// count 0.4, parts in 2).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -203,7 +229,9 @@ __device__ __forceinline__ float weight_of(const Stat& s, float top) {
 
 enum { kWhole, kNear, kFar };
 
-// Workgroups of a launch, per CU: what is resident at once.
+// Workgroups of a launch, per CU: what is resident at once. Rows of 128 need 84 registers, and three
+// workgroups a CU would fit, but read no faster than two (e4m3 76.6 us against 73.9: shorter shares,
+// more parts); two of rows of 256 take 170 us where one takes 160.
 constexpr uint32_t per_cu(uint32_t dim) { return dim <= 64 ? 4 : dim <= 128 ? 2 : 1; }
 
 // T: queries' type. E4M3: the cache holds that instead. D: head_dim rounded up to 64, 128, 256;
