@@ -47,7 +47,7 @@
 // Microseconds, and TB/s of the bytes a launch cannot do without, where a 1 GiB copy reaches 6.6: 64
 // sequences of 1k-8k tokens, 32 heads on 8 of 128 bf16, 182 (6.4); 128 of 4096, 16 on 2 of 256 f16, 160 (6.7);
 // one of 131071, 64 on 8 of 128 bf16 HND, 93 (5.8: 4 us to the first rows, 10 for the join of 64 parts);
-// 96 of 1-16384, 16 on 2 of 128 e4m3, 75 (5.2: the same, and the matrix units 20 % busy); one of 512, 9.1
+// 96 of 1-16384, 16 on 2 of 128 e4m3, 75 (5.2: the same, and the vector units 40 % busy with widening); one of 512, 9.1
 // (one round trip after another: lengths 1, table 2, rows 1.3, the wavefronts' join 0.4, parts out 1.3, the
 // count 0.4, parts in 2).
 #include <hip/hip_runtime.h>
@@ -229,7 +229,7 @@ __device__ __forceinline__ float weight_of(const Stat& s, float top) {
 
 enum { kWhole, kNear, kFar };
 
-// Workgroups of a launch, per CU: what is resident at once. Rows of 128 need 84 registers, and three
+// Workgroups of a launch, per CU: what is resident at once. Rows of 128 need 168 registers, and three
 // workgroups a CU would fit, but read no faster than two (e4m3 76.6 us against 73.9: shorter shares,
 // more parts); two of rows of 256 take 170 us where one takes 160.
 constexpr uint32_t per_cu(uint32_t dim) { return dim <= 64 ? 4 : dim <= 128 ? 2 : 1; }
@@ -626,7 +626,11 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     }
     __syncthreads();
 
-    const uint32_t quads = dim / 4, work = n_heads * quads;
+    // (made anew for every row: the compiler would otherwise work out all that follows from them, for
+    // every way below, before the first row is read: one sequence of 512 9.4 us, 9.1)
+    uint32_t tid = threadIdx.x, heads = n_heads;
+    asm volatile("" : "+v"(tid), "+s"(heads));
+    const uint32_t quads = dim / 4, work = heads * quads;
     const bool whole = n_units == units;
     const auto finish = [&](uint32_t head, uint32_t d, f32x4 o, float m, float l, bool nothing_but_inf) {
       const float inv = l == 0.0f ? (nothing_but_inf ? NAN : 0.0f) : p.v_scale / T::kTop / l;
@@ -645,7 +649,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
         p.lse[static_cast<uint64_t>(seq) * p.n_heads + head0 + head] =
             l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     };
-    for (uint32_t n = threadIdx.x; n < work; n += kThreads) {
+    for (uint32_t n = tid; n < work; n += kThreads) {
       const uint32_t head = n / quads, d = (n - head * quads) * 4;
       const uint32_t t = head / bundle, h = head - t * bundle;
       float m = -INFINITY, l = 0.0f;
@@ -682,30 +686,31 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's part is where all can see it
       __syncthreads();
       uint32_t* arrived = reinterpret_cast<uint32_t*>(lds);
-      if (threadIdx.x == 0)
+      if (tid == 0)
         *arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __syncthreads();
       const bool last = *arrived == parts - 1;
       __syncthreads();
       if (last) {
-        if (threadIdx.x == 0)   // as the next launch on this workspace wants to find it
+        if (tid == 0)   // as the next launch on this workspace wants to find it
           __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const auto slot = [&](uint32_t s) -> uint32_t {
           return (2u * ((w0 + s) * p.rows + member) + (s == 0 && behind)) * p.slot_heads;
         };
-        // Q float4s of a head by one lane, or by several (crews) that share the parts; kBatch parts
+        // Q float4s of a head (a piece of the head apart, so that lanes side by side ask for bytes side by
+        // side: one after the other 93.5 us for 131071 tokens, 92.5) by one lane, or by several (crews) that share the parts; kBatch parts
         // at a time, all asked for at once, then weighed against their maximum. Two where that saves
         // a pass (32 heads of 192, 21 parts: 35 -> 28 us for the launch), else one, whose crews have
         // less to tell one another.
         const auto join = [&](auto quads_each) {
           constexpr uint32_t Q = decltype(quads_each)::value, kBatch = 8;
-          const uint32_t per_head = dim / (4 * Q), jobs = n_heads * per_head;
+          const uint32_t per_head = dim / (4 * Q), jobs = heads * per_head;
           const uint32_t crews = jobs < kThreads ? kThreads / jobs : 1u;
           for (uint32_t n0 = 0; n0 < jobs; n0 += kThreads) {
-            const uint32_t crew = jobs < kThreads ? threadIdx.x / jobs : 0u;
-            const uint32_t n = jobs < kThreads ? threadIdx.x - crew * jobs : n0 + threadIdx.x;
+            const uint32_t crew = jobs < kThreads ? tid / jobs : 0u;
+            const uint32_t n = jobs < kThreads ? tid - crew * jobs : n0 + tid;
             const bool active = n < jobs && crew < crews;
-            const uint32_t head = n / per_head, d = (n - head * per_head) * (4 * Q);
+            const uint32_t head = n / per_head, d = (n - head * per_head) * 4, apart = dim / Q;
             float m = -INFINITY, l = 0.0f;
             bool inf = false;
             f32x4 o[Q] = {};
@@ -720,7 +725,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
                 st[k] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, is ? at * 8u : kNowhere, 0, kShared);
 #pragma unroll
                 for (uint32_t x = 0; x < Q; ++x)
-                  v[k][x] = __builtin_amdgcn_raw_buffer_load_b128(part_o, is ? (at * dim + d) * 4u + x * 16u : kNowhere, 0, kShared);
+                  v[k][x] = __builtin_amdgcn_raw_buffer_load_b128(part_o, is ? (at * dim + d + x * apart) * 4u : kNowhere, 0, kShared);
               }
               float up = m;
 #pragma unroll
@@ -750,8 +755,8 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
               Stat* mls = reinterpret_cast<Stat*>(lds + kThreads * 4 * Q);
               if (active && crew != 0) {
 #pragma unroll
-                for (uint32_t x = 0; x < Q; ++x) os[Q * threadIdx.x + x] = o[x];
-                mls[threadIdx.x] = Stat{m, l == 0.0f && inf ? -1.0f : l};
+                for (uint32_t x = 0; x < Q; ++x) os[Q * tid + x] = o[x];
+                mls[tid] = Stat{m, l == 0.0f && inf ? -1.0f : l};
               }
               __syncthreads();
               if (active && crew == 0)
@@ -768,7 +773,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
             }
             if (active && crew == 0)
 #pragma unroll
-              for (uint32_t x = 0; x < Q; ++x) finish(head, d + 4 * x, o[x], m, l, inf);
+              for (uint32_t x = 0; x < Q; ++x) finish(head, d + x * apart, o[x], m, l, inf);
           }
         };
         if (D > 64 && work >= kThreads)
