@@ -82,9 +82,9 @@ struct DecodeParams {
   uint8_t* out;
   int64_t out_token, out_head;
   float* lse;
-  float* part_o;       // [workgroup][first, last][head][head_dim]: sums not yet divided
-  float2* part_ml;     // [workgroup][first, last][head]: maximum (times log2 e), sum
-  uint32_t* counters;  // [workgroup]: parts of the row that starts in it that have been left
+  float* part_o;       // [workgroup][first, last, joined][head][head_dim]: sums not yet divided
+  float2* part_ml;     // [workgroup][first, last, joined][head]: maximum (times log2 e), sum
+  uint32_t* counters;  // [step][workgroup]: parts, of those that begin with its own, that have been left
   uint64_t block_magic;
   uint32_t visible_max, ntpb, n_blocks, n_seqs, n_heads, head_dim, window;
   uint32_t group, spread, head_rows, rows, teams, slot_heads;
@@ -217,6 +217,13 @@ __device__ __forceinline__ uint32_t units_of(const DecodeParams& p, int32_t raw)
   return (len - (start & ~(kTile - 1)) + kStep - 1) / kStep;
 }
 
+// A row's parts are joined in two steps where they are more than kFan and, together, more than kAlone float4s: one
+// workgroup reads some 25 GB/s of them. One / two steps, microseconds: 2 sequences of 65000, 64 heads on one of
+// 128, 212 / 67; one of 131071, 128 on 8 of 128 (64 parts of 512) 127 / 107; 4 of 9343, 32 on 2 of 192 (33 of 768)
+// 31.1 / 30.0; but 64 parts of 256 92.4 / 93.5, 16 of 384 15.4 / 16.1. The code of it slows launches
+// that do not need it (e4m3 74.2 / 75.6, 512 tokens 9.1 / 9.8), so that it is a kernel of its own, taken where
+// equally long sequences would be split that far; each of the two is right for any lengths.
+constexpr uint32_t kFan = 8, kAlone = 20480;
 // One part's statistics of a head. sum < 0 stands for "scores were there, all of them minus
 // infinity": that softmax is NaN, while a head that saw no token at all gives zeros.
 struct Stat {
@@ -225,6 +232,14 @@ struct Stat {
 // (the maximum passes over NaN: a part of nothing but NaN has no maximum, and a NaN sum)
 __device__ __forceinline__ float weight_of(const Stat& s, float top) {
   return s.max != -INFINITY ? __builtin_amdgcn_exp2f(s.max - top) : s.sum != s.sum ? s.sum : 0.0f;
+}
+
+// The launch's arguments, loaded where this is called and not kept in registers from the start.
+typedef __attribute__((address_space(4))) const DecodeParams* params_t;
+__device__ __forceinline__ params_t arguments() {
+  uint64_t at = reinterpret_cast<uint64_t>(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(at));
+  return (params_t)at;
 }
 
 enum { kWhole, kNear, kFar };
@@ -236,8 +251,8 @@ constexpr uint32_t per_cu(uint32_t dim) { return dim <= 64 ? 4 : dim <= 128 ? 2 
 
 // T: queries' type. E4M3: the cache holds that instead. D: head_dim rounded up to 64, 128, 256;
 // EXACT: it is D. PAGES: kWhole where 16 tokens that start at a multiple of 16 lie within one page;
-// else, of a cache whose offsets fit 32 bits, kNear, or kFar.
-template <class T, bool E4M3, int D, bool EXACT, int PAGES>
+// else, of a cache whose offsets fit 32 bits, kNear, or kFar. TWO: parts may be joined in two steps.
+template <class T, bool E4M3, int D, bool EXACT, int PAGES, bool TWO>
 __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const DecodeParams p) {
   constexpr int CB = E4M3 ? 1 : 2;                         // bytes of a cached element
   constexpr int KP = D * CB / 64;                          // 16-byte pieces of a K row per lane
@@ -649,6 +664,12 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
         p.lse[static_cast<uint64_t>(seq) * p.n_heads + head0 + head] =
             l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     };
+    const auto leave = [&](uint32_t at, uint32_t d, f32x4 o, float m, float l, bool nothing_but_inf) {
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), part_o, (at * dim + d) * 4u, 0, kShared);
+      if (d == 0)
+        __builtin_amdgcn_raw_buffer_store_b64(
+            u32x2{__float_as_uint(m), __float_as_uint(l == 0.0f && nothing_but_inf ? -1.0f : l)}, part_ml, at * 8u, 0, kShared);
+    };
     for (uint32_t n = tid; n < work; n += kThreads) {
       const uint32_t head = n / quads, d = (n - head * quads) * 4;
       const uint32_t t = head / bundle, h = head - t * bundle;
@@ -668,13 +689,89 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       if (whole) {
         finish(head, d, o, m, l, inf);
       } else {
-        const uint32_t at = (2u * blockIdx.x + (u != u_begin)) * p.slot_heads + head;
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), part_o, (at * dim + d) * 4u, 0, kShared);
-        if (d == 0)
-          __builtin_amdgcn_raw_buffer_store_b64(
-              u32x2{__float_as_uint(m), __float_as_uint(l == 0.0f && inf ? -1.0f : l)}, part_ml, at * 8u, 0, kShared);
+        const uint32_t at = (3u * blockIdx.x + (u != u_begin)) * p.slot_heads + head;
+        leave(at, d, o, m, l, inf);
       }
     }
+    // Q float4s of a head (a piece of the head apart, so that lanes side by side ask for bytes side by
+    // side: one after the other 93.5 us for 131071 tokens, 92.5) by one lane, or by several (crews) that share the parts; kBatch parts
+    // at a time, all asked for at once, then weighed against their maximum. Two where that saves
+    // a pass (32 heads of 192, 21 parts: 35 -> 28 us for the launch), else one, whose crews have
+    // less to tell one another.
+    const auto join = [&](auto quads_each, uint32_t count, const auto& slot, const auto& sink) {
+      constexpr uint32_t Q = decltype(quads_each)::value, kBatch = 8;
+      const uint32_t per_head = dim / (4 * Q), jobs = heads * per_head;
+      const uint32_t crews = jobs < kThreads ? kThreads / jobs : 1u;
+      for (uint32_t n0 = 0; n0 < jobs; n0 += kThreads) {
+        const uint32_t crew = jobs < kThreads ? tid / jobs : 0u;
+        const uint32_t n = jobs < kThreads ? tid - crew * jobs : n0 + tid;
+        const bool active = n < jobs && crew < crews;
+        const uint32_t head = n / per_head, d = (n - head * per_head) * 4, apart = dim / Q;
+        float m = -INFINITY, l = 0.0f;
+        bool inf = false;
+        f32x4 o[Q] = {};
+        for (uint32_t s0 = crew; s0 < count; s0 += kBatch * crews) {
+          u32x2 st[kBatch];
+          u32x4 v[kBatch][Q];
+#pragma unroll
+          for (uint32_t k = 0; k < kBatch; ++k) {
+            // a part that is none is behind the buffer's end: zeros come back
+            const uint32_t s = s0 + k * crews, at = slot(s) + head;
+            const bool is = active && s < count;
+            st[k] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, is ? at * 8u : kNowhere, 0, kShared);
+#pragma unroll
+            for (uint32_t x = 0; x < Q; ++x)
+              v[k][x] = __builtin_amdgcn_raw_buffer_load_b128(part_o, is ? (at * dim + d + x * apart) * 4u : kNowhere, 0, kShared);
+          }
+          float up = m;
+#pragma unroll
+          for (uint32_t k = 0; k < kBatch; ++k) {
+            if (s0 + k * crews >= count) st[k].x = __float_as_uint(-INFINITY);
+            up = fmaxf(up, __uint_as_float(st[k].x));
+          }
+          const float f_old = weight_of(Stat{m, l}, up);
+          if (f_old != 1.0f) {
+            l *= f_old;
+#pragma unroll
+            for (uint32_t x = 0; x < Q; ++x) o[x] *= f_old;
+          }
+#pragma unroll
+          for (uint32_t k = 0; k < kBatch; ++k) {
+            const Stat part_st = {__uint_as_float(st[k].x), __uint_as_float(st[k].y)};
+            const float f = weight_of(part_st, up);
+            inf = inf || part_st.sum < 0.0f;
+            l += f != 0.0f ? f * part_st.sum : 0.0f;
+#pragma unroll
+            for (uint32_t x = 0; x < Q; ++x) o[x] += f * __builtin_bit_cast(f32x4, v[k][x]);
+          }
+          m = up;
+        }
+        if (crews > 1) {
+          f32x4* os = reinterpret_cast<f32x4*>(lds);
+          Stat* mls = reinterpret_cast<Stat*>(lds + kThreads * 4 * Q);
+          if (active && crew != 0) {
+#pragma unroll
+            for (uint32_t x = 0; x < Q; ++x) os[Q * tid + x] = o[x];
+            mls[tid] = Stat{m, l == 0.0f && inf ? -1.0f : l};
+          }
+          __syncthreads();
+          if (active && crew == 0)
+            for (uint32_t t = 1; t < crews; ++t) {
+              const uint32_t at = t * jobs + n;
+              const Stat other = mls[at];
+              const float up = fmaxf(m, other.max), f_old = weight_of(Stat{m, l}, up), f = weight_of(other, up);
+              inf = inf || other.sum < 0.0f;
+              l = (f_old != 0.0f ? f_old * l : 0.0f) + (f != 0.0f ? f * other.sum : 0.0f);
+#pragma unroll
+              for (uint32_t x = 0; x < Q; ++x) o[x] = (f_old != 0.0f ? f_old : 0.0f) * o[x] + f * os[Q * at + x];
+              m = up;
+            }
+        }
+        if (active && crew == 0)
+#pragma unroll
+          for (uint32_t x = 0; x < Q; ++x) sink(head, d + x * apart, o[x], m, l, inf);
+      }
+    };
     if (!whole) {
       // the last workgroup of this row to get here joins the parts, in their order: those of the
       // teams w0 ... w1, the first's behind whatever it did before
@@ -682,104 +779,59 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       const uint32_t w1 = static_cast<uint32_t>(((before + units) * n_teams - 1) / total);
       const uint32_t parts = w1 - w0 + 1;
       const bool behind = w0 * total / n_teams < before;
-      uint32_t* counter = p.counters + w0 * p.rows + member;
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's part is where all can see it
-      __syncthreads();
-      uint32_t* arrived = reinterpret_cast<uint32_t*>(lds);
-      if (tid == 0)
-        *arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      __syncthreads();
-      const bool last = *arrived == parts - 1;
-      __syncthreads();
-      if (last) {
-        if (tid == 0)   // as the next launch on this workspace wants to find it
+      const auto last_of = [&](uint32_t* counter, uint32_t count) -> bool {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wavefront's part is where all can see it
+        __syncthreads();
+        uint32_t* arrived = reinterpret_cast<uint32_t*>(lds);
+        if (tid == 0)
+          *arrived = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        const bool last = *arrived == count - 1;
+        __syncthreads();
+        if (last && tid == 0)   // as the next launch on this workspace wants to find it
           __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const auto slot = [&](uint32_t s) -> uint32_t {
-          return (2u * ((w0 + s) * p.rows + member) + (s == 0 && behind)) * p.slot_heads;
-        };
-        // Q float4s of a head (a piece of the head apart, so that lanes side by side ask for bytes side by
-        // side: one after the other 93.5 us for 131071 tokens, 92.5) by one lane, or by several (crews) that share the parts; kBatch parts
-        // at a time, all asked for at once, then weighed against their maximum. Two where that saves
-        // a pass (32 heads of 192, 21 parts: 35 -> 28 us for the launch), else one, whose crews have
-        // less to tell one another.
-        const auto join = [&](auto quads_each) {
-          constexpr uint32_t Q = decltype(quads_each)::value, kBatch = 8;
-          const uint32_t per_head = dim / (4 * Q), jobs = heads * per_head;
-          const uint32_t crews = jobs < kThreads ? kThreads / jobs : 1u;
-          for (uint32_t n0 = 0; n0 < jobs; n0 += kThreads) {
-            const uint32_t crew = jobs < kThreads ? tid / jobs : 0u;
-            const uint32_t n = jobs < kThreads ? tid - crew * jobs : n0 + tid;
-            const bool active = n < jobs && crew < crews;
-            const uint32_t head = n / per_head, d = (n - head * per_head) * 4, apart = dim / Q;
-            float m = -INFINITY, l = 0.0f;
-            bool inf = false;
-            f32x4 o[Q] = {};
-            for (uint32_t s0 = crew; s0 < parts; s0 += kBatch * crews) {
-              u32x2 st[kBatch];
-              u32x4 v[kBatch][Q];
-#pragma unroll
-              for (uint32_t k = 0; k < kBatch; ++k) {
-                // a part that is none is behind the buffer's end: zeros come back
-                const uint32_t s = s0 + k * crews, at = slot(s) + head;
-                const bool is = active && s < parts;
-                st[k] = __builtin_amdgcn_raw_buffer_load_b64(part_ml, is ? at * 8u : kNowhere, 0, kShared);
-#pragma unroll
-                for (uint32_t x = 0; x < Q; ++x)
-                  v[k][x] = __builtin_amdgcn_raw_buffer_load_b128(part_o, is ? (at * dim + d + x * apart) * 4u : kNowhere, 0, kShared);
-              }
-              float up = m;
-#pragma unroll
-              for (uint32_t k = 0; k < kBatch; ++k) {
-                if (s0 + k * crews >= parts) st[k].x = __float_as_uint(-INFINITY);
-                up = fmaxf(up, __uint_as_float(st[k].x));
-              }
-              const float f_old = weight_of(Stat{m, l}, up);
-              if (f_old != 1.0f) {
-                l *= f_old;
-#pragma unroll
-                for (uint32_t x = 0; x < Q; ++x) o[x] *= f_old;
-              }
-#pragma unroll
-              for (uint32_t k = 0; k < kBatch; ++k) {
-                const Stat part_st = {__uint_as_float(st[k].x), __uint_as_float(st[k].y)};
-                const float f = weight_of(part_st, up);
-                inf = inf || part_st.sum < 0.0f;
-                l += f != 0.0f ? f * part_st.sum : 0.0f;
-#pragma unroll
-                for (uint32_t x = 0; x < Q; ++x) o[x] += f * __builtin_bit_cast(f32x4, v[k][x]);
-              }
-              m = up;
-            }
-            if (crews > 1) {
-              f32x4* os = reinterpret_cast<f32x4*>(lds);
-              Stat* mls = reinterpret_cast<Stat*>(lds + kThreads * 4 * Q);
-              if (active && crew != 0) {
-#pragma unroll
-                for (uint32_t x = 0; x < Q; ++x) os[Q * tid + x] = o[x];
-                mls[tid] = Stat{m, l == 0.0f && inf ? -1.0f : l};
-              }
-              __syncthreads();
-              if (active && crew == 0)
-                for (uint32_t t = 1; t < crews; ++t) {
-                  const uint32_t at = t * jobs + n;
-                  const Stat other = mls[at];
-                  const float up = fmaxf(m, other.max), f_old = weight_of(Stat{m, l}, up), f = weight_of(other, up);
-                  inf = inf || other.sum < 0.0f;
-                  l = (f_old != 0.0f ? f_old * l : 0.0f) + (f != 0.0f ? f * other.sum : 0.0f);
-#pragma unroll
-                  for (uint32_t x = 0; x < Q; ++x) o[x] = (f_old != 0.0f ? f_old : 0.0f) * o[x] + f * os[Q * at + x];
-                  m = up;
-                }
-            }
-            if (active && crew == 0)
-#pragma unroll
-              for (uint32_t x = 0; x < Q; ++x) finish(head, d + x * apart, o[x], m, l, inf);
+        return last;
+      };
+      if (!TWO || parts <= kFan || parts * work <= kAlone) {
+        if (last_of(p.counters + w0 * p.rows + member, parts)) {
+          const auto slot = [&](uint32_t s) -> uint32_t {
+            return (3u * ((w0 + s) * p.rows + member) + (s == 0 && behind)) * p.slot_heads;
+          };
+          if (D > 64 && work >= kThreads)
+            join(std::integral_constant<uint32_t, D == 64 ? 1 : 2>(), parts, slot, finish);
+          else
+            join(std::integral_constant<uint32_t, 1>(), parts, slot, finish);
+        }
+      } else if constexpr (TWO) {
+        // in two steps: `fan` neighbouring parts by the last of their workgroups, what those leave by
+        // the last of these
+        const params_t a = arguments();
+        const uint32_t rows = a->rows, slot_heads = a->slot_heads;
+        uint32_t fan = kFan;
+        while (fan * fan < parts) fan *= 2;
+        const uint32_t from = (team - w0) / fan * fan, some = parts - from < fan ? parts - from : fan;
+        const uint32_t sum_slot = (3u * ((w0 + from) * rows + member) + 2u) * slot_heads;
+        bool second = false;
+        for (uint32_t count = some;;) {
+          if (count > 1) {
+            if (!last_of(a->counters + (second ? a->teams + w0 : w0 + from) * rows + member, count)) break;
+            join(std::integral_constant<uint32_t, D == 64 ? 1 : 2>(), count,
+                 [&](uint32_t s) -> uint32_t {
+                   const uint32_t at = second ? s * fan : from + s;
+                   const uint32_t which = second && at + 1 < parts ? 2u : at == 0 && behind ? 1u : 0u;
+                   return (3u * ((w0 + at) * rows + member) + which) * slot_heads;
+                 },
+                 [&](uint32_t head, uint32_t d, f32x4 o, float m, float l, bool nothing_but_inf) {
+                   if (second)
+                     finish(head, d, o, m, l, nothing_but_inf);
+                   else
+                     leave(sum_slot + head, d, o, m, l, nothing_but_inf);
+                 });
           }
-        };
-        if (D > 64 && work >= kThreads)
-          join(std::integral_constant<uint32_t, D == 64 ? 1 : 2>());
-        else
-          join(std::integral_constant<uint32_t, 1>());
+          if (second) break;
+          second = true;
+          count = (parts + fan - 1) / fan;
+        }
       }
     }
     u += n_units;
@@ -799,25 +851,34 @@ struct Launch {
   dim3 grid;
   uint32_t lds;
   int pages;
+  bool two_steps;
   hipStream_t stream;
 };
 
-template <class T, bool E4M3, int D, bool EXACT>
+template <class T, bool E4M3, int D, bool EXACT, bool TWO>
 void launch_pages(const DecodeParams& p, const Launch& l) {
   if (l.pages == kWhole)
-    decode_kernel<T, E4M3, D, EXACT, kWhole><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+    decode_kernel<T, E4M3, D, EXACT, kWhole, TWO><<<l.grid, kThreads, l.lds, l.stream>>>(p);
   else if (l.pages == kNear)
-    decode_kernel<T, E4M3, D, EXACT, kNear><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+    decode_kernel<T, E4M3, D, EXACT, kNear, TWO><<<l.grid, kThreads, l.lds, l.stream>>>(p);
   else
-    decode_kernel<T, E4M3, D, EXACT, kFar><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+    decode_kernel<T, E4M3, D, EXACT, kFar, TWO><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+}
+
+template <class T, bool E4M3, int D, bool EXACT>
+void launch_join(const DecodeParams& p, const Launch& l) {
+  if (l.two_steps)
+    launch_pages<T, E4M3, D, EXACT, true>(p, l);
+  else
+    launch_pages<T, E4M3, D, EXACT, false>(p, l);
 }
 
 template <class T, bool E4M3, int D>
 void launch_exact(const DecodeParams& p, const Launch& l) {
   if (p.head_dim == D)
-    launch_pages<T, E4M3, D, true>(p, l);
+    launch_join<T, E4M3, D, true>(p, l);
   else
-    launch_pages<T, E4M3, D, false>(p, l);
+    launch_join<T, E4M3, D, false>(p, l);
 }
 
 template <class T, bool E4M3>
@@ -858,8 +919,8 @@ struct kvt_decode {
 
   uint32_t n_wgs = 0, teams = 0;
   bool pairs = false;   // neighbouring KV heads may be taken side by side
-  uint64_t ml_at() const { return round_up(n_wgs * 2ull * slot_heads * (pairs ? 2 : 1) * layout.head_dim * 4, 256); }
-  uint64_t counters_at() const { return round_up(ml_at() + n_wgs * 2ull * slot_heads * (pairs ? 2 : 1) * 8, 256); }
+  uint64_t ml_at() const { return round_up(n_wgs * 3ull * slot_heads * (pairs ? 2 : 1) * layout.head_dim * 4, 256); }
+  uint64_t counters_at() const { return round_up(ml_at() + n_wgs * 3ull * slot_heads * (pairs ? 2 : 1) * 8, 256); }
 
   int workspace(hipStream_t s, unsigned long long capture, uint8_t** out) {
     const std::thread::id me = s == hipStreamPerThread ? std::this_thread::get_id() : std::thread::id();
@@ -924,7 +985,7 @@ int kvt_decode_create(int device, const kvt_kv_layout* layout, uint32_t dtype, u
     const uint32_t row = layout->head_dim * dtype_bytes(layout->dtype);
     d->pairs = d->group <= 16 && layout->n_kv_heads >= 4 && layout->n_kv_heads % 2 == 0 && row <= 256 &&
                layout->head_stride == row;
-    const uint64_t counters = d->n_wgs;
+    const uint64_t counters = 2ull * d->n_wgs;
     d->ws_bytes = round_up(d->counters_at() + counters * 4, 256);
     d->owners.resize(n_workspaces);
     DeviceGuard g;
@@ -1059,7 +1120,9 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     const int pages = d->layout.ntpb % 16 == 0 && d->layout.token_stride <= (1u << 27) ? kWhole
                       : d->extent < kNowhere                                          ? kNear
                                                                                       : kFar;
-    const Launch l{dim3(wgs), std::max<uint32_t>(meet, kThreads * 40), pages, s};
+    const uint32_t split = p.teams / n_seqs;   // parts of a sequence, of equally long ones
+    const bool two_steps = split > kFan && static_cast<uint64_t>(split) * p.slot_heads * dim / 4 > kAlone;
+    const Launch l{dim3(wgs), std::max<uint32_t>(meet, kThreads * 40), pages, two_steps, s};
     if (d->dtype == KVT_DTYPE_BF16) {
       if (e4m3) launch_dim<Bf16, true>(p, l);
       else launch_dim<Bf16, false>(p, l);

@@ -338,6 +338,22 @@ def test_long_sequences_split_over_the_device():
             assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+@pytest.mark.parametrize("kind,cache_kind,layout,lens,heads,kv_heads,dim,block", [
+    ("bf16", "bf16", "flash", [20011], 64, 1, 128, 16), ("f16", "f16", "hnd", [9001, 0, 7], 33, 1, 256, 16),
+    ("bf16", "e4m3", "ragged", [12345, 3000], 128, 2, 64, 5), ("bf16", "bf16", "flash", [33000], 32, 4, 128, 16),
+    ("bf16", "bf16", "pages", [1100, 8192], 70, 1, 192, 64)])
+def test_many_heads_split_so_far_that_parts_are_joined_in_two_steps(kind, cache_kind, layout, lens, heads, kv_heads, dim,
+                                                                    block):
+    c = Case(kind, cache_kind, layout, lens, heads, kv_heads, dim, block, seed=25)
+    op, exact = c.operator(), c.exact()
+    first = c.check(op, exact)
+    for max_len in (max(lens), 1, 2000):
+        c.check(op, exact, max_len=max_len)
+    for _ in range(4):
+        again = c.check(op, exact)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 @pytest.mark.parametrize("n", [63, 64, 65, 700])
 def test_many_short_sequences(n):
     rng = np.random.default_rng(12)
