@@ -220,7 +220,7 @@ __device__ __forceinline__ uint32_t units_of(const DecodeParams& p, int32_t raw)
 // A row's parts are joined in two steps where they are more than kFan and, together, more than kAlone float4s: one
 // workgroup reads some 25 GB/s of them. One / two steps, microseconds: 2 sequences of 65000, 64 heads on one of
 // 128, 212 / 67; one of 131071, 128 on 8 of 128 (64 parts of 512) 127 / 107; 4 of 9343, 32 on 2 of 192 (33 of 768)
-// 31.1 / 30.0; but 64 parts of 256 92.4 / 93.5, 16 of 384 15.4 / 16.1. The code of it slows launches
+// 31.1 / 30.0 (not kept for such heads); but 64 parts of 256 92.4 / 93.5, 16 of 384 15.4 / 16.1. The code of it slows launches
 // that do not need it (e4m3 74.2 / 75.6, 512 tokens 9.1 / 9.8), so that it is a kernel of its own, taken where
 // equally long sequences would be split that far; each of the two is right for any lengths.
 constexpr uint32_t kFan = 8, kAlone = 20480;
@@ -694,8 +694,8 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       }
     }
     // Q float4s of a head (a piece of the head apart, so that lanes side by side ask for bytes side by
-    // side: one after the other 93.5 us for 131071 tokens, 92.5) by one lane, or by several (crews) that share the parts; kBatch parts
-    // at a time, all asked for at once, then weighed against their maximum. Two where that saves
+    // side: one after the other 93.5 us for 131071 tokens, 92.5) by one lane, or by several (crews) that
+    // share the parts; kBatch parts at a time, all asked for at once, then weighed against their maximum. Two where that saves
     // a pass (32 heads of 192, 21 parts: 35 -> 28 us for the launch), else one, whose crews have
     // less to tell one another.
     const auto join = [&](auto quads_each, uint32_t count, const auto& slot, const auto& sink) {
@@ -855,30 +855,29 @@ struct Launch {
   hipStream_t stream;
 };
 
-template <class T, bool E4M3, int D, bool EXACT, bool TWO>
-void launch_pages(const DecodeParams& p, const Launch& l) {
-  if (l.pages == kWhole)
-    decode_kernel<T, E4M3, D, EXACT, kWhole, TWO><<<l.grid, kThreads, l.lds, l.stream>>>(p);
-  else if (l.pages == kNear)
-    decode_kernel<T, E4M3, D, EXACT, kNear, TWO><<<l.grid, kThreads, l.lds, l.stream>>>(p);
-  else
-    decode_kernel<T, E4M3, D, EXACT, kFar, TWO><<<l.grid, kThreads, l.lds, l.stream>>>(p);
-}
-
 template <class T, bool E4M3, int D, bool EXACT>
-void launch_join(const DecodeParams& p, const Launch& l) {
-  if (l.two_steps)
-    launch_pages<T, E4M3, D, EXACT, true>(p, l);
-  else
-    launch_pages<T, E4M3, D, EXACT, false>(p, l);
+void launch_pages(const DecodeParams& p, const Launch& l) {
+  if (l.pages == kNear) {
+    decode_kernel<T, E4M3, D, EXACT, kNear, false><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+  } else if (l.pages == kFar) {
+    decode_kernel<T, E4M3, D, EXACT, kFar, false><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+  } else {
+    // (two steps for the usual head sizes and pages alone: every kernel takes its seconds to compile)
+    if constexpr (EXACT)
+      if (l.two_steps) {
+        decode_kernel<T, E4M3, D, EXACT, kWhole, true><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+        return;
+      }
+    decode_kernel<T, E4M3, D, EXACT, kWhole, false><<<l.grid, kThreads, l.lds, l.stream>>>(p);
+  }
 }
 
 template <class T, bool E4M3, int D>
 void launch_exact(const DecodeParams& p, const Launch& l) {
   if (p.head_dim == D)
-    launch_join<T, E4M3, D, true>(p, l);
+    launch_pages<T, E4M3, D, true>(p, l);
   else
-    launch_join<T, E4M3, D, false>(p, l);
+    launch_pages<T, E4M3, D, false>(p, l);
 }
 
 template <class T, bool E4M3>
@@ -1120,8 +1119,9 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     const int pages = d->layout.ntpb % 16 == 0 && d->layout.token_stride <= (1u << 27) ? kWhole
                       : d->extent < kNowhere                                          ? kNear
                                                                                       : kFar;
-    const uint32_t split = p.teams / n_seqs;   // parts of a sequence, of equally long ones
-    const bool two_steps = split > kFan && static_cast<uint64_t>(split) * p.slot_heads * dim / 4 > kAlone;
+    // parts of a sequence, of equally long ones (14 of 1536 float4s: one step 28.6 us, two 30.3)
+    const uint32_t split = p.teams / n_seqs;
+    const bool two_steps = split > 2 * kFan && static_cast<uint64_t>(split) * p.slot_heads * dim / 4 > kAlone;
     const Launch l{dim3(wgs), std::max<uint32_t>(meet, kThreads * 40), pages, two_steps, s};
     if (d->dtype == KVT_DTYPE_BF16) {
       if (e4m3) launch_dim<Bf16, true>(p, l);
