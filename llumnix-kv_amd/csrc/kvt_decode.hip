@@ -446,9 +446,12 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
           } else if constexpr (PAGES == kNear) {
             const uint32_t at = __shfl(off[s], row) + k_lane[j];
             load_to_lds(rows, EXACT || k_lane[j] != kNowhere ? at : kNowhere, to);
-          } else if (EXACT || k_lane[j] != kNowhere) {
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)(kbase + __shfl(off[s], row) + k_lane[j]), to, 16, 0, kStreamed);
+          } else {
+            // (by all lanes: one whose own piece lies behind the head's end still tells others where a row is)
+            const int64_t at = __shfl(off[s], row);
+            if (EXACT || k_lane[j] != kNowhere)
+              __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kbase + at + k_lane[j]), to,
+                                               16, 0, kStreamed);
           }
         }
       }

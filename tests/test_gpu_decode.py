@@ -413,6 +413,51 @@ def test_pages_of_a_cache_beyond_32_bits_that_end_inside_a_tile():
     hold(out, lse, exact, "bf16")
 
 
+@pytest.fixture(scope="module")
+def far_bytes():
+    """5 GiB in which every element of every type is NaN."""
+    return torch.full((5 << 30,), 0xFF, device="cuda", dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("kind,cache_kind", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "e4m3"), ("f16", "e4m3")])
+@pytest.mark.parametrize("dim,block", [(16, 24), (16, 1), (32, 5), (48, 5), (64, 3), (80, 24), (96, 5), (112, 7), (128, 5),
+                                       (144, 24), (192, 5), (240, 3)])
+def test_head_sizes_in_a_cache_beyond_32_bits(far_bytes, kind, cache_kind, dim, block):
+    """Pages 128 MiB apart that end inside a tile: every row of K and V, of every head size."""
+    n_blocks, kv, heads, size = 40, 2, 6, 1 if cache_kind == "e4m3" else 2
+    far_bytes.fill_(0xFF)
+    handle = kvt_amd.Cache(0, [[far_bytes]], [far_bytes.numel()])
+    row = dim * size
+    strides = (128 << 20, block * kv * row, kv * row, row)
+    lay = kvt_amd.KvLayout(None, cache_kind, n_blocks, block, kv, dim, strides=strides)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim * 100 + block)
+    lens = [block * 33 - block // 2, 1, block * 4]
+    ids = torch.randperm(n_blocks, generator=g, device="cuda")[:38].split([33, 1, 4])
+    tables = np.full((3, 33), -1, dtype=np.int32)
+    where = []
+    for b, (n, mine) in enumerate(zip(lens, ids)):
+        tables[b, :len(mine)] = mine.cpu().numpy()
+        t = torch.arange(n, device="cuda")
+        where.append(mine[t // block] * block + t % block)
+    where = torch.cat(where)
+    k, v = (torch.randn((sum(lens), kv, dim), generator=g, device="cuda").to(oc.torch_type(kind)) for _ in range(2))
+    q = (2 * torch.randn((3, heads, dim), generator=g, device="cuda")).to(oc.torch_type(kind))
+    kvt_amd.kv_append(handle, 0, lay, k, v, where)
+    plain, at = [], (where.cpu().numpy() // block, where.cpu().numpy() % block)
+    for rows in (k, v):
+        pages = np.zeros((n_blocks, block, kv, dim))
+        pages[at] = oc.wide(rows.to(oc.torch_type(cache_kind)))
+        plain.append(pages)
+    out, lse = torch.empty_like(q), torch.empty((3, heads), device="cuda")
+    op = kvt_amd.DecodeAttention(0, lay, kind, heads, max_seqs=3)
+    exact = oc.decode_exact(oc.wide(q), *plain, tables, lens, block, dim ** -0.5)
+    for max_len in (0, 1):
+        op.run(handle, 0, q, torch.from_numpy(tables).cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda"), out,
+               lse=lse, max_len=max_len)
+        hold(out, lse, exact, kind)
+
+
 def test_offsets_beyond_32_bits():
     """Pages at the far end of a cache of 9 GiB, K and V more than 4 GiB apart."""
     block, kv, dim, n_blocks = 16, 2, 64, 1 << 21
