@@ -954,7 +954,8 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
  * already), with a window the last `window` of them. Token t lies in block block_tables[b][t / ntpb].
  * Not seen either: tokens behind the table's table_blocks columns, and those of a block id outside
  * [0, n_blocks). A sequence that sees no token (a padding row: length 0 or negative) gets zeros and
- * an lse of minus infinity. Rows of the cache that are not seen may hold anything, NaN included.
+ * an lse of minus infinity. Rows of the cache that are not seen may hold anything, NaN included. What is
+ * infinite or NaN in V of a token that is seen makes that element of the output so, however small its weight.
  * Scores, weights, sums and the maximum are held in 32 bits, the weights take part in the product
  * with V as two 16-bit values each; every output is rounded once. The same call gives the same
  * bits each time; the other sequences of a batch and max_len move a sequence's result within the

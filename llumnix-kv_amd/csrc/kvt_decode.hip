@@ -16,12 +16,13 @@
 // Weights are split into two 16-bit values each (the weight cut off and what that left, rounded),
 // so that the product with V loses nothing that counts beside the output's own rounding: rounding
 // them once costs as much error as the output's rounding does, the second product costs a few
-// matrix instructions in a kernel that is bound by HBM. Both values are positive (the rest at
-// least the smallest positive number), so that an infinity in V times a weight is that infinity,
-// as in the formula, and not the difference of two. For f16 the weights are taken times 2^15, which
-// makes its smallest positive number 2^-39 of the largest weight: 2^-24 of it, for each of the many
+// matrix instructions in a kernel that is bound by HBM. Both values are at least the smallest
+// positive number, so that an infinity in V times a weight is that infinity, as in the formula, and
+// neither the difference of two nor zero times one. For f16 the weights are taken times 2^16, which
+// makes its smallest positive number 2^-40 of the largest weight: 2^-24 of it, for each of the many
 // small weights of a long sequence in which one token stands out, would add up to more than the
-// output's own rounding.
+// output's own rounding. (The largest weights, cut off to f16's largest number of 65504, leave the rest
+// of 65536 as any other.)
 //
 // An 8-bit cache is widened on load: every e4m3 value is a bf16 and an f16 value.
 //
@@ -63,6 +64,7 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
@@ -102,12 +104,13 @@ struct Bf16 {
   static __device__ __forceinline__ uint32_t widen(uint32_t e4m3) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(e4m3, 1.0f, HIGH));
   }
-  // two values cut off to this type, its smallest positive number worth adding, and what the
-  // largest weight is in the product with V
+  // two values cut off to this type, its smallest positive number (here of the normal ones) and
+  // the bits of two of them, and what the largest weight is in the product with V
   static __device__ __forceinline__ uint32_t cut(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
   }
   static constexpr float kLeast = 0x1p-126f, kTop = 1.0f;
+  static constexpr uint32_t kLeastTwice = 0x00800080u;
 };
 struct F16 {
   typedef _Float16 x8 __attribute__((ext_vector_type(8)));
@@ -122,7 +125,8 @@ struct F16 {
   static __device__ __forceinline__ uint32_t cut(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
   }
-  static constexpr float kLeast = 0x1p-24f, kTop = 0x1p15f;
+  static constexpr float kLeast = 0x1p-24f, kTop = 0x1p16f;
+  static constexpr uint32_t kLeastTwice = 0x00010001u;
 };
 
 // N pieces of 16 bytes from LDS, once all but the newest `NEWER` vector memory operations are done:
@@ -233,6 +237,10 @@ struct Stat {
 __device__ __forceinline__ float weight_of(const Stat& s, float top) {
   return s.max != -INFINITY ? __builtin_amdgcn_exp2f(s.max - top) : s.sum != s.sum ? s.sum : 0.0f;
 }
+// What sums of V are multiplied with for a weight: never zero, which would make an infinity NaN. One in a
+// row that is seen then comes through wherever the sequence is split, as it does within a tile. (A NaN weight
+// ends here, and makes the row NaN by its sum.)
+__device__ __forceinline__ float carried(float weight) { return fmaxf(weight, 0x1p-126f); }
 
 // The launch's arguments, loaded where this is called and not kept in registers from the start.
 typedef __attribute__((address_space(4))) const DecodeParams* params_t;
@@ -554,8 +562,8 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       for (int i = 0; i < 8; ++i) high = fmaxf(high, sc[i >> 2][i & 3]);
       high = over_tokens_max(high);
       if (__any(high != top)) {
-        // a head with nothing but minus infinity so far: exp2(-inf - 0) = 0
-        const float shrink = __builtin_amdgcn_exp2f(top - (high == -INFINITY ? 0.0f : high));
+        // a head with nothing but minus infinity so far: exp2(-inf - 0) = 0, of a sum of zero
+        const float shrink = carried(__builtin_amdgcn_exp2f(top - (high == -INFINITY ? 0.0f : high)));
         sum *= shrink;
 #pragma unroll
         for (int x = 0; x < NA; ++x) acc[x] *= shrink;
@@ -569,7 +577,9 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
         float a = __builtin_amdgcn_exp2f(sc[s][r] - ref), b = __builtin_amdgcn_exp2f(sc[s][r + 1] - ref);
         sum += a + b;
         a *= T::kTop, b *= T::kTop;
-        const uint32_t hi = T::cut(a, b);
+        // (positive numbers, and NaN above them, are in the order of their bits)
+        const uint32_t hi = __builtin_bit_cast(
+            uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, T::cut(a, b)), __builtin_bit_cast(u16x2, T::kLeastTwice)));
         const f32x2 kept = __builtin_convertvector(__builtin_bit_cast(typename T::x2, hi), f32x2);
         const f32x2 rest = {fmaxf(a - kept.x, T::kLeast), fmaxf(b - kept.y, T::kLeast)};
         ph[i] = hi;
@@ -684,10 +694,8 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
         const Stat s = stats[w * 16 + h];
         const float f = weight_of(s, m);
         inf = inf || s.sum < 0.0f;
-        if (f != 0.0f) {
-          l += f * s.sum;
-          o += f * *reinterpret_cast<const f32x4*>(part + (w * bundle + h) * kRow + d);
-        }
+        if (f != 0.0f) l += f * s.sum;
+        o += carried(f) * *reinterpret_cast<const f32x4*>(part + (w * bundle + h) * kRow + d);
       }
       if (whole) {
         finish(head, d, o, m, l, inf);
@@ -736,7 +744,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
           if (f_old != 1.0f) {
             l *= f_old;
 #pragma unroll
-            for (uint32_t x = 0; x < Q; ++x) o[x] *= f_old;
+            for (uint32_t x = 0; x < Q; ++x) o[x] *= carried(f_old);
           }
 #pragma unroll
           for (uint32_t k = 0; k < kBatch; ++k) {
@@ -745,7 +753,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
             inf = inf || part_st.sum < 0.0f;
             l += f != 0.0f ? f * part_st.sum : 0.0f;
 #pragma unroll
-            for (uint32_t x = 0; x < Q; ++x) o[x] += f * __builtin_bit_cast(f32x4, v[k][x]);
+            for (uint32_t x = 0; x < Q; ++x) o[x] += carried(f) * __builtin_bit_cast(f32x4, v[k][x]);
           }
           m = up;
         }
@@ -766,7 +774,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
               inf = inf || other.sum < 0.0f;
               l = (f_old != 0.0f ? f_old * l : 0.0f) + (f != 0.0f ? f * other.sum : 0.0f);
 #pragma unroll
-              for (uint32_t x = 0; x < Q; ++x) o[x] = (f_old != 0.0f ? f_old : 0.0f) * o[x] + f * os[Q * at + x];
+              for (uint32_t x = 0; x < Q; ++x) o[x] = carried(f_old) * o[x] + carried(f) * os[Q * at + x];
               m = up;
             }
         }

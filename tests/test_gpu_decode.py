@@ -268,6 +268,46 @@ def test_infinities_and_nan_that_are_seen_follow_the_formula():
     hold(out[1:2], lse[1:2], exact, "bf16")
 
 
+@pytest.mark.parametrize("kind,cache_kind,value", [("bf16", "bf16", "inf"), ("f16", "f16", "-inf"), ("bf16", "bf16", "nan"),
+                                                   ("bf16", "e4m3", "nan"), ("f16", "e4m3", "nan")])
+@pytest.mark.parametrize("at,high", [(5, 6), (5, 40), (40, 5), (5, 133), (133, 5), (5, 590), (590, 5), (300, 301)])
+def test_infinities_and_nan_in_v_come_through_wherever_a_sequence_is_split(kind, cache_kind, value, at, high):
+    """One token's weight leaves nothing of the others' in 32 bits (their scores are 2000 below), in the same tile, in
+    another wavefront's, in a later tile, in another workgroup's share: what is not finite in another's V shows."""
+    c = Case(kind, cache_kind, "flash", [600, 77], 4, 1, 64, 16, seed=26)
+    k, v = (x.view(c.cache_type) for x in oc.kv_views("flash", c.cache))
+    page = lambda t: (int(c.tables[0, t // 16]), t % 16)  # noqa: E731
+    c.q[0, :, 0] = 80.0
+    k[page(high)][0, 0] = 200.0
+    v[page(at)][0, 7] = float(value)
+    row = oc.wide(v[page(high)])[0]
+    rest = oc.decode_exact(oc.wide(c.q)[1:], *c.plain, c.tables[1:], [77], 16, 64 ** -0.5)
+    for max_len in (0, 1):
+        out, lse = c.buffers()
+        c.operator().run(c.handle, 0, c.q, c.d_tables, c.d_lens, out, lse=lse, max_len=max_len)
+        got = oc.wide(out)[0]
+        assert np.array_equal(got[:, 7], np.full(4, float(value)), equal_nan=True), (max_len, got[:, 7])
+        # the others: the row of the one token that counts, its sums rounded a few times in 32 bits
+        got, want = np.delete(got, 7, axis=1), np.delete(row, 7)
+        rel, floor = oc.HALF_STEP[kind]
+        assert (np.abs(got - want) <= rel * np.abs(want) + floor + 2.0 ** -15 * np.abs(want)).all()
+        hold(out[1:], lse[1:], rest, kind)
+
+
+@pytest.mark.parametrize("at", [3, 9000, 20010])
+def test_infinities_in_v_come_through_the_join_in_two_steps(at):
+    c = Case("bf16", "bf16", "flash", [20011], 64, 1, 128, 16, seed=27)
+    k, v = (x.view(torch.bfloat16) for x in oc.kv_views("flash", c.cache))
+    c.q[0, :, 0] = 80.0
+    k[int(c.tables[0, 10001 // 16]), 10001 % 16][0, 0] = 300.0
+    v[int(c.tables[0, at // 16]), at % 16][0, 7] = float("inf")
+    for max_len in (0, 1):
+        out, lse = c.buffers()
+        c.operator().run(c.handle, 0, c.q, c.d_tables, c.d_lens, out, lse=lse, max_len=max_len)
+        got = oc.wide(out)[0]
+        assert np.isposinf(got[:, 7]).all() and np.isfinite(np.delete(got, 7, axis=1)).all()
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_every_8_bit_value_is_itself(kind):
     """One token: the output is its row of V, times the scale; NaN included. As keys: scores that are
