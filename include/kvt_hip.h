@@ -981,7 +981,8 @@ int kvt_decode_create(int device, const kvt_kv_layout* layout, uint32_t dtype, u
                       uint32_t n_workspaces, kvt_decode** out);
 void kvt_decode_destroy(kvt_decode* d);
 /* Gives back what `stream` holds: its eager workspace and those of the captures made on it. Call
- * it when the stream's launches have run and its graphs are gone (before the stream is destroyed). */
+ * it when the stream's launches have run and its graphs are gone (before the stream is destroyed).
+ * hipStreamPerThread stands for the calling thread's stream alone, here as in launches. */
 int kvt_decode_release(kvt_decode* d, void* stream);
 /* q, out: rows as in kvt_rotary_apply (q, out, lse and, for what is written, the cache's tensor share no bytes). block_tables: int32, row b
  * at b * table_stride entries; seq_lens: int32. max_len: the longest length of the batch as far as

@@ -932,8 +932,13 @@ struct kvt_decode {
   uint64_t ml_at() const { return round_up(n_wgs * 3ull * slot_heads * (pairs ? 2 : 1) * layout.head_dim * 4, 256); }
   uint64_t counters_at() const { return round_up(ml_at() + n_wgs * 3ull * slot_heads * (pairs ? 2 : 1) * 8, 256); }
 
+  // hipStreamPerThread is one handle for a stream of every thread: what tells them apart.
+  static std::thread::id thread_of(hipStream_t s) {
+    return s == hipStreamPerThread ? std::this_thread::get_id() : std::thread::id();
+  }
+
   int workspace(hipStream_t s, unsigned long long capture, uint8_t** out) {
-    const std::thread::id me = s == hipStreamPerThread ? std::this_thread::get_id() : std::thread::id();
+    const std::thread::id me = thread_of(s);
     std::lock_guard<std::mutex> lock(mu);
     size_t free = owners.size();
     for (size_t i = 0; i < owners.size(); ++i) {
@@ -1032,8 +1037,10 @@ void kvt_decode_destroy(kvt_decode* d) {
 int kvt_decode_release(kvt_decode* d, void* stream) {
   if (!d) return fail(KVT_ERR_INVALID, "kvt_decode_release: null argument");
   std::lock_guard<std::mutex> lock(d->mu);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const std::thread::id me = kvt_decode::thread_of(s);
   for (kvt_decode::Owner& o : d->owners)
-    if (o.taken && o.stream == static_cast<hipStream_t>(stream)) o = kvt_decode::Owner{};
+    if (o.taken && o.stream == s && o.thread == me) o = kvt_decode::Owner{};
   return KVT_OK;
 }
 

@@ -2,6 +2,8 @@
 64 bits on the CPU: types, layouts, head counts and sizes, lengths around every boundary, pages that
 end inside a tile, windows, caps, rows that see nothing, rows that must not be looked at, splits,
 streams and graphs. Needs a real MI355X."""
+import concurrent.futures
+
 import numpy as np
 import pytest
 
@@ -551,6 +553,34 @@ def test_streams_have_workspaces_of_their_own():
     op.release(streams[0].cuda_stream)
     op.run(a.handle, 0, a.q, a.d_tables, a.d_lens, out, lse=lse)
     hold(out, lse, exact[0], "bf16")
+
+
+def test_releasing_the_per_thread_stream_gives_back_this_threads_workspace_alone():
+    """hipStreamPerThread is one handle for a stream of every thread."""
+    per_thread = 2
+    c = Case("bf16", "bf16", "flash", [3000, 20], 8, 2, 64, 16, seed=28)
+    op, exact = c.operator(workspaces=2), c.exact()
+    buffers = [c.buffers() for _ in range(4)]
+    torch.cuda.synchronize()
+
+    def launch(n, stream):
+        out, lse = buffers[n]
+        op.run(c.handle, 0, c.q, c.d_tables, c.d_lens, out, lse=lse, stream=stream)
+        torch.cuda.synchronize()
+
+    def elsewhere(n):
+        with concurrent.futures.ThreadPoolExecutor(1) as pool:
+            pool.submit(launch, n, per_thread).result()
+
+    elsewhere(0)                                             # another thread's stream takes one workspace
+    launch(1, per_thread)                                    # and this thread's the other
+    op.release(per_thread)
+    launch(2, checkers.side_stream().cuda_stream)            # finds the one that this thread has given back
+    with pytest.raises(kvt_amd.KvtError) as e:
+        launch(3, checkers.side_stream().cuda_stream)        # and no second one
+    assert e.value.code == ERR_INVALID
+    for out, lse in buffers[:3]:
+        hold(out, lse, exact, "bf16")
 
 
 def test_graphs_replay_with_new_lengths_and_tables():
