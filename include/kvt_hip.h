@@ -914,7 +914,8 @@ void kvt_rotary_destroy(kvt_rotary* r);
  * elements of dtype (BF16, F16 or F32; head_dim >= rotary_dim, up to 256 and of any size
  * otherwise). Rows at token * token_stride + head * head_stride bytes, elements of a row next to
  * each other. out == x with the same strides rotates in place; an output that otherwise shares
- * bytes with x is refused, and so are output strides that let rows meet. positions: int64, on the
+ * bytes with x is refused, as is one that interleaves with x at other strides than x's (rows of one
+ * wider tensor, q = w[:, :, 0] and out = w[:, :, 1], may), and so are output strides that let rows meet. positions: int64, on the
  * device, may be negative. Pointers and strides that are multiples of 16 bytes, with head_dim and
  * rotary_dim multiples of 16, take the vector path, anything aligned to the element a slower one. */
 int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void* x,

@@ -109,12 +109,32 @@ int check_apart(const Rows& in, uint32_t in_heads, const Rows& out, uint32_t out
   const uint64_t a = reinterpret_cast<uintptr_t>(in.ptr), b = reinterpret_cast<uintptr_t>(out.ptr);
   if (a + (n_tokens - 1) * in.token_stride + in_token <= b || b + (n_tokens - 1) * out.token_stride + out_token <= a)
     return KVT_OK;
-  if (in_place && a == b && in.token_stride == out.token_stride && in.head_stride == out.head_stride) return KVT_OK;
+  // (a stride of one token or one head is no stride)
+  const bool same_tokens = n_tokens == 1 || in.token_stride == out.token_stride;
+  const bool same_heads = in_heads == 1 || out_heads == 1 || in.head_stride == out.head_stride;
+  if (in_place && a == b && same_tokens && in_heads == out_heads && same_heads) return KVT_OK;
   const uint64_t stride = out.token_stride;
   if (in.token_stride == stride && in_token <= stride && out_token <= stride) {
     // both repeat with the same period: apart when one period's intervals are
     const uint64_t gap = a >= b ? (a - b) % stride : (stride - (b - a) % stride) % stride;   // a behind b
     if (gap >= out_token && gap + in_token <= stride) return KVT_OK;
+  }
+  if (same_tokens && same_heads) {
+    // rows interleave head by head (or token by token within a head): those of two tokens dt apart and two
+    // heads dh apart meet where |a - b + dt token_stride + dh head_stride| < row_bytes
+    typedef __int128 wide;
+    const wide t_stride = n_tokens == 1 ? 0 : in.token_stride, most = n_tokens - 1, row = row_bytes;
+    const wide h_stride = in_heads > 1 ? in.head_stride : out_heads > 1 ? out.head_stride : 0;
+    const auto floored = [](wide n, wide d) { return n / d - (n % d < 0); };
+    bool meet = false;
+    for (wide dh = -(static_cast<wide>(out_heads) - 1); dh < in_heads && !meet; ++dh) {
+      const wide c = static_cast<wide>(a) - static_cast<wide>(b) + dh * h_stride;
+      if (t_stride == 0)
+        meet = -row < c && c < row;
+      else
+        meet = std::max(floored(-row - c, t_stride) + 1, -most) <= std::min(floored(row - c - 1, t_stride), most);
+    }
+    if (!meet) return KVT_OK;
   }
   return fail(KVT_ERR_INVALID, text(who, std::string("the output shares bytes with ") + what +
                                              " without being the same rows"));

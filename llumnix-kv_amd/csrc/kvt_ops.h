@@ -38,7 +38,8 @@ int check_rows(const Rows& r, uint64_t n_tokens, uint32_t n_heads, uint64_t row_
                uint32_t elem, bool written, const char* who, const char* what, uint64_t* span);
 // Refuses rows that are read (`what`) where they share bytes with rows that are written by the
 // same launch, unless they are the very same rows and `in_place` allows that. Slices of one wider
-// tensor that interleave without sharing a byte are told apart.
+// tensor that interleave without sharing a byte are told apart, token by token or (with equal strides)
+// head by head.
 int check_apart(const Rows& in, uint32_t in_heads, const Rows& out, uint32_t out_heads, uint64_t n_tokens,
                 uint64_t row_bytes, bool in_place, const char* who, const char* what);
 

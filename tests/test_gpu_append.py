@@ -221,6 +221,28 @@ def test_append_saturates_and_keeps_nan_like_the_converting_pack():
     assert torch.equal(cache[:, 0, 0, 0].flatten(), want) and torch.equal(cache[:, 0, 1, 0].flatten(), want)
 
 
+@pytest.mark.parametrize("n", [1, 5, 300])
+def test_a_projection_that_is_fused_head_by_head(n):
+    """[tokens, heads, 3, dim] with its queries rotated in place beside keys and values."""
+    g = _gen(21)
+    w = _normal((n, 6, 3, 64), "bf16", g)
+    before = w.clone()
+    q, k, v = w[:, :, 0], w[:, :, 1], w[:, :, 2]
+    r, pos = kvt_amd.Rotary(64), torch.randint(0, 9999, (n,), generator=g, device="cuda")
+    lay = kvt_amd.KvLayout(kvt_amd.SHAPE_FLASH, "bf16", 30, 16, 6, 64)
+    slots = torch.randperm(480, generator=g, device="cuda")[:n].contiguous()
+    caches = [torch.zeros((2, 30, 16, 6, 64), device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    handles = [kvt_amd.Cache(0, [[c]], [c.numel() * 2]) for c in caches]
+    q_out = torch.empty((n, 6, 64), device="cuda", dtype=torch.bfloat16)
+    kvt_amd.kv_append(handles[0], 0, lay, k.contiguous(), v.contiguous(), slots, rotary=r, positions=pos, q=q.contiguous(),
+                      q_out=q_out)
+    kvt_amd.kv_append(handles[1], 0, lay, k, v, slots, rotary=r, positions=pos, q=q, q_out=q)
+    assert torch.equal(caches[0], caches[1]) and torch.equal(q, q_out) and torch.equal(w[:, :, 1:], before[:, :, 1:])
+    # from one third of it to another
+    r.apply(before[:, :, 0], pos, before[:, :, 2])
+    assert torch.equal(before[:, :, 2], q_out) and torch.equal(before[:, :, 1], k)
+
+
 def test_no_tokens_is_no_launch():
     cache = torch.zeros((2, 4, 16, 2, 64), device="cuda", dtype=torch.bfloat16)
     handle = kvt_amd.Cache(0, [[cache]], [cache.numel() * 2])

@@ -140,6 +140,48 @@ def test_calls_that_are_right_need_a_device():
     assert _apply(r, x=P + 1024, x_tok=2048, out=P, out_tok=2048) == ctypes_defs.ERR_NO_DEVICE
 
 
+@pytest.mark.skipif(kvt_amd.device_count() > 0, reason="this check is for machines without a GPU")
+def test_rows_of_one_wider_tensor_that_share_no_byte_are_told_apart():
+    r, free = kvt_amd.Rotary(64), ctypes_defs.ERR_NO_DEVICE
+    heads = dict(x_tok=2048, x_head=256, out_tok=2048, out_head=256)     # [tokens, 8, 2, 64]: x = w[:, :, 0]
+    for off in (128, -128, 128 + 3 * 256, 2048 - 128, 128 - 5 * 2048, 70 * 2048 - 128):
+        assert _apply(r, out=P + off, **heads) == free, off
+    for off in (126, 2, -2, 256, -256, 130, 2048, -63 * 2048, 63 * 2048 + 7 * 256 + 126):
+        assert _apply(r, out=P + off, **heads) == ERR_INVALID, off
+    assert _apply(r, out=P + 63 * 2048 + 7 * 256 + 128, **heads) == free
+    # heads in front of tokens, [8, 2, 64, 64]: x = w[:, 0]
+    heads = dict(x_tok=128, x_head=16384, out_tok=128, out_head=16384)
+    assert _apply(r, out=P + 8192, **heads) == free and _apply(r, out=P - 8192, **heads) == free
+    for off in (8192 - 128, 8192 + 128, 8190, -8194, 128, 16384):
+        assert _apply(r, out=P + off, **heads) == ERR_INVALID, off
+    # interleaved at other strides: not worked out
+    assert _apply(r, out=P + 128, x_tok=2048, x_head=256, out_tok=4096, out_head=256) == ERR_INVALID
+    # strides of one token or of one head are none
+    assert _apply(r, out=P, n=1, out_tok=4096) == free and _apply(r, out=P + 128, n=1, x_head=256, out_head=256) == free
+    assert _apply(r, out=P, heads=1, x_head=2, out_head=6, x_tok=256, out_tok=256) == free
+    assert _apply(r, out=P + 64, n=1, out_tok=4096) == ERR_INVALID
+    assert _apply(r, out=P + 64, heads=1, x_head=2, x_tok=256, out_tok=256) == ERR_INVALID
+
+
+@pytest.mark.skipif(kvt_amd.device_count() > 0, reason="this check is for machines without a GPU")
+def test_rows_at_the_same_strides_are_refused_exactly_where_they_share_bytes():
+    r, rng, seen = kvt_amd.Rotary(2), np.random.default_rng(31), set()
+    for _ in range(4000):
+        n, heads = (int(x) for x in rng.integers(1, 6, 2))
+        strides = sorted(int(x) * 2 for x in rng.integers(2, 24, 2))
+        tok, head = (strides if rng.random() < 0.5 else strides[::-1])
+        off = 2 * int(rng.integers(-80, 80))
+        rows = np.array([t * tok + h * head for t in range(n) for h in range(heads)])
+        if np.diff(np.sort(rows)).min(initial=4) < 4:
+            continue                                         # rows of the output itself meet
+        got = _apply(r, x=P, x_tok=tok, x_head=head, out=P + off, out_tok=tok, out_head=head, n=n, heads=heads, dim=2)
+        meet = (np.abs(rows[:, None] - (rows + off)[None]) < 4).any() and off != 0
+        refusals = ERR_INVALID if meet else ctypes_defs.ERR_NO_DEVICE
+        assert got == refusals or "overlap" in kvt_amd.lib().kvt_last_error().decode(), (n, heads, tok, head, off, got)
+        seen.add((got, bool(meet)))
+    assert (ERR_INVALID, True) in seen and (ctypes_defs.ERR_NO_DEVICE, False) in seen
+
+
 def _append(layout, rotary, **kw):
     a = dict(dtype=0, k=P, k_tok=4096, k_head=256, v=P + 2048, v_tok=4096, v_head=256, q=4 * P, q_tok=8192, q_head=256,
              q_heads=32, q_out=8 * P, qo_tok=8192, qo_head=256, positions=POS, slots=2 * POS, n=8, k_scale=1.0,
@@ -173,6 +215,17 @@ def test_append_refuses_on_the_host():
     fused = dict(q=P, q_tok=12288, q_out=P, qo_tok=12288, k=P + 8192, k_tok=12288, v=P + 10240, v_tok=12288)
     assert _append(lay, r, **fused) == ERR_INVALID and b"null cache" in said()
     assert _append(lay, r, **dict(fused, k=P + 8000)) == ERR_INVALID and b"shares bytes with k" in said()
+
+
+def test_append_takes_queries_rotated_in_place_in_a_projection_that_is_fused_head_by_head():
+    lay, r = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128), kvt_amd.Rotary(128)
+    w = dict(q=P, q_tok=6144, q_head=768, q_heads=8, q_out=P, qo_tok=6144, qo_head=768, k=P + 256, k_tok=6144, k_head=768,
+             v=P + 512, v_tok=6144, v_head=768)                          # [tokens, 8, 3, 128]
+    said = lambda: kvt_amd.lib().kvt_last_error()  # noqa: E731
+    assert _append(lay, r, **w) == ERR_INVALID and b"null cache" in said()
+    assert _append(lay, r, **dict(w, n=1)) == ERR_INVALID and b"null cache" in said()
+    assert _append(lay, r, **dict(w, k=P + 254)) == ERR_INVALID and b"shares bytes with k" in said()
+    assert _append(lay, r, **dict(w, v=P + 768)) == ERR_INVALID and b"shares bytes with v" in said()
 
 
 @pytest.mark.parametrize("strides", [(0, 1 << 16, 256, 4096), (65536, 256, 256, 4096), (65536, 1 << 22, 255, 4096),
