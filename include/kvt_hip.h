@@ -858,7 +858,8 @@ int kvt_object_ring_stats(kvt_object_ring* r, kvt_object_ring_counters* out);
  * cache as it is registered for the transfer (kvt_cache) and the layouts of its cache shapes, run
  * on the caller's stream, allocate nothing, synchronise nothing and can be captured into a hipGraph.
  * Device arrays (positions, slots, block tables, lengths) are read by the kernels alone; a value
- * in them that names no row of the cache is skipped there as stated below, never followed. */
+ * in them that names no row of the cache is skipped there as stated below, never followed. They share no
+ * bytes with what a call writes. */
 
 enum { KVT_DTYPE_BF16 = 0, KVT_DTYPE_F16 = 1, KVT_DTYPE_F32 = 2, KVT_DTYPE_E4M3 = 3 };
 

@@ -420,6 +420,7 @@ int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void
     if (int rc = check_apart(in, n_heads, to, n_heads, n_tokens, head_dim * elem, true, who, "x")) return rc;
     if (in_span != 0 && (!positions || reinterpret_cast<uintptr_t>(positions) & 7u))
       return fail(KVT_ERR_INVALID, "kvt_rotary_apply: positions are null or not aligned");
+    if (int rc = check_distinct(who, {out, out_span, "out"}, {{positions, 8 * n_tokens, "positions"}})) return rc;
     if (int rc = check_device(device)) return rc;
     if (in_span == 0) return KVT_OK;
     DeviceGuard g;
@@ -482,18 +483,21 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
       return fail(KVT_ERR_INVALID, "kvt_kv_append: slots are null or not aligned");
     if (n_tokens != 0 && rotary && (!positions || reinterpret_cast<uintptr_t>(positions) & 7u))
       return fail(KVT_ERR_INVALID, "kvt_kv_append: positions are null or not aligned");
+    const Span slot_array{slots, 8 * n_tokens, "slots"}, position_array{positions, rotary ? 8 * n_tokens : 0, "positions"};
+    if (int rc = check_distinct(who, {q_out, qo_span, "q_out"}, {slot_array, position_array})) return rc;
     uint8_t* base = nullptr;
     if (int rc = check_cache_layer(cache, layer, layout, extent, who, &base)) return rc;
     if (n_tokens == 0) return KVT_OK;
     if (int rc = check_distinct(who, {base, extent, "the cache's tensor"},
-                                {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"}}))
+                                {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"},
+                                 slot_array, position_array}))
       return rc;
     DeviceGuard g;
     if (int rc = g.enter(cache->device)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (!being_captured(s))
       if (int rc = check_spans(who, {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"},
-                                     {slots, 8 * n_tokens, "slots"}, {positions, rotary ? 8 * n_tokens : 0, "positions"}}))
+                                     slot_array, position_array}))
         return rc;
     RotateParams p{};
     p.q = static_cast<const uint8_t*>(q), p.k = static_cast<const uint8_t*>(k), p.v = static_cast<const uint8_t*>(v);

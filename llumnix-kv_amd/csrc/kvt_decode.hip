@@ -1074,6 +1074,11 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     if (int rc = check_distinct(who, {base, d->extent, "the cache's tensor"}, {outs, lses})) return rc;
     if (int rc = check_distinct(who, lses, {outs, {q, q_span, "q"}})) return rc;
     if (table_stride > (1ull << 40)) return fail(KVT_ERR_INVALID, "kvt_decode_attention: table_stride out of range");
+    // (workgroups that read different lengths would wait for different numbers of parts)
+    const Span lens{seq_lens, 4ull * n_seqs, "seq_lens"};
+    const Span tables{block_tables, table_blocks ? 4 * ((n_seqs - 1) * table_stride + table_blocks) : 0, "block_tables"};
+    if (int rc = check_distinct(who, outs, {lens, tables})) return rc;
+    if (int rc = check_distinct(who, lses, {lens, tables})) return rc;
     DeviceGuard g;
     if (int rc = g.enter(d->device)) return rc;
     const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -1081,11 +1086,7 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     unsigned long long capture = 0;
     if (hipStreamIsCapturing(s, &cap) != hipSuccess) (void)hipGetLastError();
     if (cap == hipStreamCaptureStatusNone) {
-      if (int rc = check_spans(
-              who, {{q, q_span, "q"}, outs, {seq_lens, 4ull * n_seqs, "seq_lens"},
-                    {block_tables, table_blocks ? 4 * ((n_seqs - 1) * table_stride + table_blocks) : 0, "block_tables"},
-                    lses}))
-        return rc;
+      if (int rc = check_spans(who, {{q, q_span, "q"}, outs, lens, tables, lses})) return rc;
     } else if (hipStreamGetCaptureInfo(s, &cap, &capture) != hipSuccess || capture == 0) {
       (void)hipGetLastError();
       return fail(KVT_ERR_HIP, "kvt_decode_attention: the stream's capture cannot be told apart");

@@ -292,6 +292,21 @@ def test_append_refusals_that_need_a_cache():
     assert not cache.any()
 
 
+def test_slots_and_positions_inside_the_cache_are_refused():
+    cache = torch.zeros((2, 4, 16, 2, 64), device="cuda", dtype=torch.bfloat16)
+    handle = kvt_amd.Cache(0, [[cache]], [cache.numel() * 2])
+    lay = kvt_amd.KvLayout(kvt_amd.SHAPE_FLASH, "bf16", 4, 16, 2, 64)
+    rows, slots = torch.ones((3, 2, 64), device="cuda", dtype=torch.bfloat16), torch.arange(3, device="cuda")
+    inside = cache.view(torch.int64).flatten()[-3:]
+    r = kvt_amd.Rotary(64)
+    for kw in (dict(slots=inside), dict(slots=slots, rotary=r, positions=inside)):
+        with pytest.raises(kvt_amd.KvtError) as e:
+            kvt_amd.kv_append(handle, 0, lay, rows, rows, **kw)
+        assert e.value.code == ERR_INVALID and "the cache's tensor shares bytes" in str(e.value)
+    torch.cuda.synchronize()
+    assert not cache.any()
+
+
 def test_captured_append_reads_its_arrays_anew_on_every_replay():
     st = checkers.side_stream()
     g = _gen(9)

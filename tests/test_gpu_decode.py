@@ -635,6 +635,21 @@ def test_two_graphs_at_once():
             hold(out, lse, exact, "bf16")
 
 
+def test_tables_and_lengths_inside_what_is_written_are_refused():
+    c = Case("bf16", "bf16", "flash", [100, 64, 40], 4, 2, 64, 16, seed=30)
+    op = c.operator()
+    out, lse = c.buffers()
+    as_int = out.view(torch.int32).flatten()
+    cols = c.tables.shape[1]
+    for lens, tables, sums in ((as_int[-3:], c.d_tables, None), (c.d_lens, as_int[5:5 + 3 * cols].view(3, cols), None),
+                               (lse.view(torch.int32).flatten()[:3], c.d_tables, lse),
+                               (c.d_lens, lse.view(torch.int32).flatten()[-3 * 2:].view(3, 2), lse)):
+        with pytest.raises(kvt_amd.KvtError) as e:
+            op.run(c.handle, 0, c.q, tables, lens, out, lse=sums)
+        assert e.value.code == ERR_INVALID and "shares bytes" in str(e.value)
+    c.check(op, c.exact())
+
+
 def test_refusals():
     c = Case("bf16", "bf16", "flash", [100, 64], 4, 2, 64, 16, seed=18)
     out, lse = c.buffers()

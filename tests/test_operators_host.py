@@ -217,6 +217,20 @@ def test_append_refuses_on_the_host():
     assert _append(lay, r, **dict(fused, k=P + 8000)) == ERR_INVALID and b"shares bytes with k" in said()
 
 
+def test_index_arrays_inside_what_is_written_are_refused():
+    lay, r = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128), kvt_amd.Rotary(128)
+    said = lambda: kvt_amd.lib().kvt_last_error()  # noqa: E731
+    last = 8 * P + 7 * 8192 + 31 * 256 + 256                 # behind the last row of q_out
+    for at in (8 * P - 56, 8 * P, 8 * P + 4096, last - 8):
+        assert _append(lay, r, slots=at) == ERR_INVALID and b"q_out shares bytes with slots" in said()
+        assert _append(lay, r, positions=at) == ERR_INVALID and b"q_out shares bytes with positions" in said()
+    for at in (8 * P - 64, last):
+        assert _append(lay, r, slots=at, positions=at) == ERR_INVALID and b"null cache" in said()
+    r = kvt_amd.Rotary(64)
+    for at in (2 * P, 2 * P - 8 * 63, 2 * P + 63 * 1024 + 1016):
+        assert _apply(r, positions=at) == ERR_INVALID and b"out shares bytes with positions" in said()
+
+
 def test_append_takes_queries_rotated_in_place_in_a_projection_that_is_fused_head_by_head():
     lay, r = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128), kvt_amd.Rotary(128)
     w = dict(q=P, q_tok=6144, q_head=768, q_heads=8, q_out=P, qo_tok=6144, qo_head=768, k=P + 256, k_tok=6144, k_head=768,
