@@ -16,12 +16,12 @@ _types = {}          # "int32", "int64" and the codes above -> torch dtype; torc
 
 
 def _torch_types():
-    """Filled by the first call that is given a tensor: this package does without torch."""
+    """Made by the first call that is given a tensor (this package does without torch), and put in place
+    whole: another thread finds all of it or nothing."""
+    global _types
     import torch
     named = {0: torch.bfloat16, 1: torch.float16, 2: torch.float32}
-    _types.update(named)
-    _types.update({t: code for code, t in named.items()})
-    _types.update(int32=torch.int32, int64=torch.int64)
+    _types = {**named, **{t: code for code, t in named.items()}, "int32": torch.int32, "int64": torch.int64}
     return _types
 
 

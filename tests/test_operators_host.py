@@ -299,3 +299,38 @@ def test_the_binding_checks_sizes_and_types_before_the_library():
         r.apply(rows, slots[:1], rows)
     with pytest.raises(ValueError):
         r.apply(rows.transpose(1, 2), slots, rows.transpose(1, 2))
+
+
+def test_a_first_call_beside_another_threads_first_call(monkeypatch):
+    """The table of torch types is there whole or not at all, wherever the thread that makes it is held back."""
+    import threading
+
+    import torch
+    from kvt_amd import operators
+    held, go_on, done = threading.Event(), threading.Event(), threading.Event()
+
+    class Halting(dict):
+        def update(self, *args, **kw):
+            super().update(*args, **kw)
+            held.set()
+            go_on.wait(10)
+
+    monkeypatch.setattr(operators, "_types", Halting())
+    rows, slots = torch.zeros((3, 2, 64), dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int64)
+
+    def first():
+        operators._code(rows, "k")
+        held.set()
+        done.set()
+
+    thread = threading.Thread(target=first)
+    thread.start()
+    try:
+        assert held.wait(10)
+        assert operators._code(rows, "k") == 0
+        assert operators._rows(rows, "k", (3, 2, 64), 0)[1:] == (256, 128)
+        assert operators._index(slots, "slots", (3,), "int64") == slots.data_ptr()
+    finally:
+        go_on.set()
+        thread.join()
+    assert done.is_set()
