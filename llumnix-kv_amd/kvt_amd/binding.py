@@ -483,7 +483,7 @@ class Cache:
         flat = (_vp * (n_layers * n_tensors))(*[_ptr(t) for l in layers for t in l])
         cap = (_u64 * n_tensors)(*capacity)
         self.h = _vp()
-        self._keep = layers
+        self._keep, self.device = layers, device
         check(lib().kvt_cache_register(device, flat, n_layers, n_tensors, cap, C.byref(self.h)))
 
     def close(self):

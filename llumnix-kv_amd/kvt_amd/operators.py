@@ -4,11 +4,11 @@ token over them.
 
 Tensors are torch tensors on the cache's device (any strides; the elements of a row next to each
 other), `stream` a hipStream_t handle as everywhere in this package (None: the default stream).
-Sizes and types are checked here, everything else by the library."""
+Sizes, types and devices are checked here, everything else by the library."""
 import ctypes as C
 
-from . import binding
-from .binding import KvLayoutStruct, RotaryOpts, _quiet_close, check, lib
+from .binding import KvLayoutStruct, KvtError, RotaryOpts, _quiet_close, check, lib
+from .ctypes_defs import ERR_INVALID
 
 DTYPES = {"bf16": 0, "f16": 1, "f32": 2, "e4m3": 3}
 SCALINGS = {"plain": 0, "linear": 1, "bands": 2, "ramp": 3}
@@ -49,6 +49,14 @@ def _index(tensor, name, shape, kind):
     if tensor.shape != shape or tensor.dtype != _types[kind] or not tensor.is_contiguous():
         raise ValueError("%s: expected a contiguous %s tensor of shape %s" % (name, _types[kind], shape))
     return tensor.data_ptr()
+
+
+def _refuse_elsewhere(device, tensors):
+    """Refuses tensors that the device's kernels may not reach: those of another device, or in plain host
+    memory. (The library sees pointers, and inside a capture does not ask the runtime about them.)"""
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != device and not (t.get_device() < 0 and t.is_pinned()):
+            raise KvtError(ERR_INVALID, "%s and what it is used with are not on one device (%d)" % (name, device))
 
 
 class KvLayout:
@@ -105,8 +113,11 @@ class Rotary:
         code = _code(x, "x")
         x_ptr, x_t, x_h = _rows(x, "x", shape, code)
         out_ptr, out_t, out_h = _rows(out, "out", shape, code)
-        rc = lib().kvt_rotary_apply(self.h, x.get_device(), code, x_ptr, x_t, x_h, out_ptr, out_t, out_h,
-                                    _index(positions, "positions", (n,), "int64"), n, heads, dim, stream)
+        pos_ptr, device = _index(positions, "positions", (n,), "int64"), x.get_device()
+        if out.get_device() != device or positions.get_device() != device:
+            _refuse_elsewhere(device, dict(out=out, positions=positions))
+        rc = lib().kvt_rotary_apply(self.h, device, code, x_ptr, x_t, x_h, out_ptr, out_t, out_h, pos_ptr, n, heads, dim,
+                                    stream)
         if rc:
             check(rc)
         return out
@@ -140,9 +151,14 @@ def kv_append(cache, layer, layout, k, v, slots, rotary=None, positions=None, q=
         out_ptr, out_t, out_h = _rows(q_out, "q_out", (n, q_heads, dim), code)
     if positions is not None:
         pos_ptr = _index(positions, "positions", (n,), "int64")
+    slots_ptr, device = _index(slots, "slots", (n,), "int64"), cache.device
+    if k.get_device() != device or v.get_device() != device or slots.get_device() != device or (
+            q is not None and (q.get_device() != device or q_out.get_device() != device)) or (
+            positions is not None and positions.get_device() != device):
+        _refuse_elsewhere(device, dict(k=k, v=v, slots=slots, q=q, q_out=q_out, positions=positions))
     rc = lib().kvt_kv_append(cache.h, layer, layout.ref, rotary.h if rotary is not None else None, code, k_ptr, k_t, k_h,
-                             v_ptr, v_t, v_h, q_ptr, q_t, q_h, q_heads, out_ptr, out_t, out_h, pos_ptr,
-                             _index(slots, "slots", (n,), "int64"), n, k_scale, v_scale, stream)
+                             v_ptr, v_t, v_h, q_ptr, q_t, q_h, q_heads, out_ptr, out_t, out_h, pos_ptr, slots_ptr, n,
+                             k_scale, v_scale, stream)
     if rc:
         check(rc)
 
@@ -154,7 +170,7 @@ class DecodeAttention:
     def __init__(self, device, layout, dtype, n_q_heads, max_seqs, softmax_scale=None, logit_cap=0.0, window=0,
                  workspaces=4):
         self.h = C.c_void_p()
-        self.layout, self.n_q_heads, self.code = layout, n_q_heads, DTYPES[dtype]
+        self.device, self.layout, self.n_q_heads, self.code = device, layout, n_q_heads, DTYPES[dtype]
         check(lib().kvt_decode_create(device, layout.ref, self.code, n_q_heads, softmax_scale or 0.0, logit_cap,
                                       window, max_seqs, workspaces, C.byref(self.h)))
 
@@ -171,10 +187,16 @@ class DecodeAttention:
             raise ValueError("block_tables: expected int32 [%d, blocks] with contiguous rows" % n)
         q_ptr, q_t, q_h = _rows(q, "q", shape, self.code)
         out_ptr, out_t, out_h = _rows(out, "out", shape, self.code)
+        lens_ptr, lse_ptr = _index(seq_lens, "seq_lens", (n,), "int32"), None
+        if lse is not None:
+            lse_ptr = _index(lse, "lse", (n, heads), 2)
+        device = self.device
+        if q.get_device() != device or block_tables.get_device() != device or seq_lens.get_device() != device or (
+                out.get_device() != device) or (lse is not None and lse.get_device() != device):
+            _refuse_elsewhere(device, dict(q=q, block_tables=block_tables, seq_lens=seq_lens, out=out, lse=lse))
         rc = lib().kvt_decode_attention(
-            self.h, cache.h, layer, q_ptr, q_t, q_h, block_tables.data_ptr(), block_tables.stride(0), columns,
-            _index(seq_lens, "seq_lens", (n,), "int32"), n, max_len, k_scale, v_scale, out_ptr, out_t, out_h,
-            None if lse is None else _index(lse, "lse", (n, heads), 2), stream)
+            self.h, cache.h, layer, q_ptr, q_t, q_h, block_tables.data_ptr(), block_tables.stride(0), columns, lens_ptr, n,
+            max_len, k_scale, v_scale, out_ptr, out_t, out_h, lse_ptr, stream)
         if rc:
             check(rc)
         return out

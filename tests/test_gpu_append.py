@@ -307,6 +307,30 @@ def test_slots_and_positions_inside_the_cache_are_refused():
     assert not cache.any()
 
 
+def test_host_arrays_are_taken_where_the_device_can_read_them():
+    cache = torch.zeros((2, 4, 16, 2, 64), device="cuda", dtype=torch.bfloat16)
+    handle = kvt_amd.Cache(0, [[cache]], [cache.numel() * 2])
+    lay = kvt_amd.KvLayout(kvt_amd.SHAPE_FLASH, "bf16", 4, 16, 2, 64)
+    rows = _normal((3, 2, 64), "bf16", _gen(31))
+    slots = torch.tensor([5, 40, 17])
+    pinned, host = slots.pin_memory(), rows.cpu()
+    kvt_amd.kv_append(handle, 0, lay, rows, rows, pinned)
+    torch.cuda.synchronize()
+    assert torch.equal(cache[0].flatten(0, 1)[slots.cuda()], rows)
+    st, graph = checkers.side_stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):                 # also where the runtime is not asked
+        for kw in (dict(slots=slots), dict(slots=pinned, k=host)):
+            with pytest.raises(kvt_amd.KvtError) as e:
+                kvt_amd.kv_append(handle, 0, lay, **dict(dict(k=rows, v=rows), **kw), stream=st.cuda_stream)
+            assert e.value.code == ERR_INVALID
+        kvt_amd.kv_append(handle, 0, lay, rows, rows, pinned, stream=st.cuda_stream)
+    cache.zero_()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache[1].flatten(0, 1)[slots.cuda()], rows)
+
+
 def test_captured_append_reads_its_arrays_anew_on_every_replay():
     st = checkers.side_stream()
     g = _gen(9)

@@ -334,3 +334,42 @@ def test_a_first_call_beside_another_threads_first_call(monkeypatch):
         go_on.set()
         thread.join()
     assert done.is_set()
+
+
+class _On:
+    """A tensor that says it is on some device."""
+
+    def __init__(self, tensor, device):
+        self._tensor, self._device = tensor, device
+
+    def get_device(self):
+        return self._device
+
+    def __getattr__(self, name):
+        return getattr(self._tensor, name)
+
+
+def test_tensors_of_another_device_are_refused_by_the_binding():
+    import torch
+    lay, r = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 2, 64), kvt_amd.Rotary(64)
+
+    class NoCache:
+        h, device = None, 3
+
+    rows = {n: torch.zeros((3, 2, 64), dtype=torch.bfloat16) for n in ("k", "v", "q", "q_out", "out")}
+    rows.update((n, torch.zeros(3, dtype=torch.int64)) for n in ("slots", "positions"))
+    rows.update(seq_lens=torch.zeros(3, dtype=torch.int32), block_tables=torch.zeros((3, 4), dtype=torch.int32),
+                lse=torch.zeros((3, 2)))
+    attention = object.__new__(kvt_amd.DecodeAttention)
+    attention.h, attention.layout, attention.n_q_heads, attention.code, attention.device = C.c_void_p(), lay, 2, 0, 3
+    calls = [(("k", "v", "slots", "positions", "q", "q_out"), lambda kw: kvt_amd.kv_append(NoCache, 0, lay, rotary=r, **kw)),
+             (("q", "block_tables", "seq_lens", "out", "lse"), lambda kw: attention.run(NoCache, 0, **kw)),
+             (("q", "positions", "out"), lambda kw: r.apply(kw["q"], kw["positions"], kw["out"]))]
+    for names, call in calls:
+        here = {n: _On(rows[n], 3) for n in names}
+        said = _refused(ERR_INVALID, call, here) if names[0] != "q" or len(names) > 3 else ""
+        assert "device" not in said                          # all on one device: the library's own refusal (no cache)
+        for odd in names:
+            for where in (1, -1):
+                said = _refused(ERR_INVALID, call, dict(here, **{odd: _On(rows[odd], where)}))
+                assert "not on one device" in said, (odd, where, said)
