@@ -918,7 +918,9 @@ void kvt_rotary_destroy(kvt_rotary* r);
  * bytes with x is refused, as is one that interleaves with x at other strides than x's (rows of one
  * wider tensor, q = w[:, :, 0] and out = w[:, :, 1], may), and so are output strides that let rows meet. positions: int64, on the
  * device, may be negative. Pointers and strides that are multiples of 16 bytes, with head_dim and
- * rotary_dim multiples of 16, take the vector path, anything aligned to the element a slower one. */
+ * rotary_dim multiples of 16, take the vector path, anything aligned to the element a slower one. A launch
+ * has fewer than 2^32 lanes, a lane for 32 bytes of rows (2 elements on the slower path): calls of more
+ * rows are refused, here and in kvt_kv_append. */
 int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void* x,
                      uint64_t x_token_stride, uint64_t x_head_stride, void* out,
                      uint64_t out_token_stride, uint64_t out_head_stride, const int64_t* positions,

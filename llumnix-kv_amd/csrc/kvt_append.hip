@@ -54,7 +54,6 @@ struct RotateParams {
   uint32_t items, q_items, qk_items;   // per token: all, of the queries, of queries and keys
   uint32_t row_items, rot_items;       // per row; of a query or key row, the rotated ones in front
   uint32_t half, dim, ntpb;            // pairs and elements of a row
-  bool near;                           // all items of the launch are fewer than 2^32
   bool once;                           // for the launcher: more is read than kCachedInput
   float k_mul, v_mul, magnitude;
 };
@@ -189,9 +188,9 @@ template <class T, bool E4M3, int N, bool INTER, int PAIRS, bool ONCE>
 __global__ __launch_bounds__(kThreads) void rotate_append_kernel(const RotateParams p, const Turns<PAIRS> turns) {
   extern __shared__ float2 cs[];
   constexpr int kElem = Piece<T, N>::kElem;
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * kItemsPerWg;
-  const uint64_t token0 = p.near ? divided(static_cast<uint32_t>(first), p.items_magic) : first / p.items;
-  const uint32_t rem = static_cast<uint32_t>(first - token0 * p.items);
+  const uint32_t first = blockIdx.x * kItemsPerWg, tokens_before = divided(first, p.items_magic);
+  const uint32_t rem = first - tokens_before * p.items;
+  const uint64_t token0 = tokens_before;
 
   Item<T, N> it[kItemsPerLane];
 #pragma unroll
@@ -332,21 +331,25 @@ void launch_pieces(const RotateParams& p, const double* turns, bool vec, bool in
 
 struct RotateCall {
   const kvt_rotary* rotary;
-  int device;
   uint32_t dtype, head_dim, n_q_heads, n_kv_heads;
   bool e4m3;
   bool aligned;   // every pointer and stride is a multiple of 16 bytes
   hipStream_t stream;
 };
 
-// Fills in what follows from the sizes and launches. One token's items must fit 32 bits: they
-// do with at most 65536 heads of each kind.
-int launch_rotate(const RotateCall& c, RotateParams& p, const char* who) {
+struct RotateGrid {
+  uint32_t wgs, lds;
+  bool vec, inter;
+};
+
+// What follows from the sizes. One token's items must fit 32 bits: they do with at most 65536 heads
+// of each kind. A launch has fewer than 2^32 lanes.
+int size_rotate(const RotateCall& c, RotateParams& p, const char* who, RotateGrid* grid) {
   const uint32_t dim = c.rotary ? c.rotary->dim : 0, n_vec = 16 / dtype_bytes(c.dtype);
-  const bool inter = c.rotary && c.rotary->interleaved;
+  grid->inter = c.rotary && c.rotary->interleaved;
   // vectors need an even number of whole pieces in both parts of a row
-  const bool vec = c.aligned && dim % (2 * n_vec) == 0 && c.head_dim % (2 * n_vec) == 0;
-  const uint32_t n = vec ? n_vec : 1;
+  grid->vec = c.aligned && dim % (2 * n_vec) == 0 && c.head_dim % (2 * n_vec) == 0;
+  const uint32_t n = grid->vec ? n_vec : 1;
   p.half = dim / 2;
   p.dim = c.head_dim;
   p.rot_items = p.half / n;
@@ -359,28 +362,30 @@ int launch_rotate(const RotateCall& c, RotateParams& p, const char* who) {
   p.half_magic = division_magic(p.half);
   p.block_magic = division_magic(p.ntpb);
   if (c.rotary) p.magnitude = c.rotary->magnitude;
-  const double* turns = c.rotary ? c.rotary->turns : nullptr;
   const unsigned __int128 all = static_cast<unsigned __int128>(p.n_tokens) * p.items;
   const unsigned __int128 wgs = (all + kItemsPerWg - 1) / kItemsPerWg;
-  if (wgs > 0x7FFFFF00u) return fail(KVT_ERR_INVALID, std::string(who) + ": too many rows for one launch");
-  if (wgs == 0) return KVT_OK;
-  p.near = (wgs * kItemsPerWg >> 32) == 0;
+  if (wgs > 0xFFFFFFFFu / kThreads) return fail(KVT_ERR_INVALID, std::string(who) + ": too many rows for one launch");
   p.once = all * 2 * n * dtype_bytes(c.dtype) > kCachedInput;
+  grid->wgs = static_cast<uint32_t>(wgs);
   // tokens that one workgroup's items can belong to
-  const uint32_t span = (kItemsPerWg - 2) / p.items + 2;
-  const uint32_t lds = span * p.half * static_cast<uint32_t>(sizeof(float2));
-  const uint32_t grid = static_cast<uint32_t>(wgs);
+  const uint32_t span = p.items ? (kItemsPerWg - 2) / p.items + 2 : 0;
+  grid->lds = span * p.half * static_cast<uint32_t>(sizeof(float2));
+  return KVT_OK;
+}
+
+int launch_rotate(const RotateCall& c, const RotateParams& p, const RotateGrid& g, const char* who) {
+  const double* turns = c.rotary ? c.rotary->turns : nullptr;
   switch (c.dtype) {
     case KVT_DTYPE_BF16:
-      if (c.e4m3) launch_pieces<Bf16, true>(p, turns, vec, inter, grid, lds, c.stream);
-      else launch_pieces<Bf16, false>(p, turns, vec, inter, grid, lds, c.stream);
+      if (c.e4m3) launch_pieces<Bf16, true>(p, turns, g.vec, g.inter, g.wgs, g.lds, c.stream);
+      else launch_pieces<Bf16, false>(p, turns, g.vec, g.inter, g.wgs, g.lds, c.stream);
       break;
     case KVT_DTYPE_F16:
-      if (c.e4m3) launch_pieces<F16, true>(p, turns, vec, inter, grid, lds, c.stream);
-      else launch_pieces<F16, false>(p, turns, vec, inter, grid, lds, c.stream);
+      if (c.e4m3) launch_pieces<F16, true>(p, turns, g.vec, g.inter, g.wgs, g.lds, c.stream);
+      else launch_pieces<F16, false>(p, turns, g.vec, g.inter, g.wgs, g.lds, c.stream);
       break;
     default:
-      launch_pieces<F32, false>(p, turns, vec, inter, grid, lds, c.stream);
+      launch_pieces<F32, false>(p, turns, g.vec, g.inter, g.wgs, g.lds, c.stream);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return hip_fail(e, who);
@@ -421,14 +426,6 @@ int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void
     if (in_span != 0 && (!positions || reinterpret_cast<uintptr_t>(positions) & 7u))
       return fail(KVT_ERR_INVALID, "kvt_rotary_apply: positions are null or not aligned");
     if (int rc = check_distinct(who, {out, out_span, "out"}, {{positions, 8 * n_tokens, "positions"}})) return rc;
-    if (int rc = check_device(device)) return rc;
-    if (in_span == 0) return KVT_OK;
-    DeviceGuard g;
-    if (int rc = g.enter(device)) return rc;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (!being_captured(s))
-      if (int rc = check_spans(who, {{x, in_span, "x"}, {out, out_span, "out"}, {positions, 8 * n_tokens, "positions"}}))
-        return rc;
     RotateParams p{};
     p.q = static_cast<const uint8_t*>(x);
     p.q_token = x_token_stride, p.q_head = x_head_stride;
@@ -437,8 +434,18 @@ int kvt_rotary_apply(const kvt_rotary* r, int device, uint32_t dtype, const void
     p.positions = positions;
     p.n_tokens = n_tokens;
     p.ntpb = 1;
-    return launch_rotate({r, device, dtype, head_dim, n_heads, 0, false, rows_aligned16(in) && rows_aligned16(to), s},
-                         p, who);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const RotateCall call{r, dtype, head_dim, n_heads, 0, false, rows_aligned16(in) && rows_aligned16(to), s};
+    RotateGrid grid{};
+    if (int rc = size_rotate(call, p, who, &grid)) return rc;
+    if (int rc = check_device(device)) return rc;
+    if (in_span == 0) return KVT_OK;
+    DeviceGuard g;
+    if (int rc = g.enter(device)) return rc;
+    if (!being_captured(s))
+      if (int rc = check_spans(who, {{x, in_span, "x"}, {out, out_span, "out"}, {positions, 8 * n_tokens, "positions"}}))
+        return rc;
+    return launch_rotate(call, p, grid, who);
   });
 }
 
@@ -485,20 +492,6 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
       return fail(KVT_ERR_INVALID, "kvt_kv_append: positions are null or not aligned");
     const Span slot_array{slots, 8 * n_tokens, "slots"}, position_array{positions, rotary ? 8 * n_tokens : 0, "positions"};
     if (int rc = check_distinct(who, {q_out, qo_span, "q_out"}, {slot_array, position_array})) return rc;
-    uint8_t* base = nullptr;
-    if (int rc = check_cache_layer(cache, layer, layout, extent, who, &base)) return rc;
-    if (n_tokens == 0) return KVT_OK;
-    if (int rc = check_distinct(who, {base, extent, "the cache's tensor"},
-                                {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"},
-                                 slot_array, position_array}))
-      return rc;
-    DeviceGuard g;
-    if (int rc = g.enter(cache->device)) return rc;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (!being_captured(s))
-      if (int rc = check_spans(who, {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"},
-                                     slot_array, position_array}))
-        return rc;
     RotateParams p{};
     p.q = static_cast<const uint8_t*>(q), p.k = static_cast<const uint8_t*>(k), p.v = static_cast<const uint8_t*>(v);
     p.q_token = q_token_stride, p.q_head = q_head_stride;
@@ -506,7 +499,6 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
     p.v_token = v_token_stride, p.v_head = v_head_stride;
     p.q_out = static_cast<uint8_t*>(q_out);
     p.q_out_token = q_out_token_stride, p.q_out_head = q_out_head_stride;
-    p.cache = base;
     p.block_stride = layout->block_stride, p.kv_stride = layout->kv_stride;
     p.token_stride = layout->token_stride, p.head_stride = layout->head_stride;
     p.positions = positions, p.slots = slots;
@@ -515,7 +507,23 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
     p.k_mul = 1.0f / k_scale, p.v_mul = 1.0f / v_scale;
     const bool aligned = rows_aligned16(kr) && rows_aligned16(vr) &&
                          (n_q_heads == 0 || (rows_aligned16(qr) && rows_aligned16(qo)));
-    return launch_rotate({rotary, cache->device, dtype, layout->head_dim, n_q_heads, heads, e4m3, aligned, s}, p, who);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    const RotateCall call{rotary, dtype, layout->head_dim, n_q_heads, heads, e4m3, aligned, s};
+    RotateGrid grid{};
+    if (int rc = size_rotate(call, p, who, &grid)) return rc;
+    if (int rc = check_cache_layer(cache, layer, layout, extent, who, &p.cache)) return rc;
+    if (n_tokens == 0) return KVT_OK;
+    if (int rc = check_distinct(who, {p.cache, extent, "the cache's tensor"},
+                                {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"},
+                                 slot_array, position_array}))
+      return rc;
+    DeviceGuard g;
+    if (int rc = g.enter(cache->device)) return rc;
+    if (!being_captured(s))
+      if (int rc = check_spans(who, {{k, k_span, "k"}, {v, v_span, "v"}, {q, q_span, "q"}, {q_out, qo_span, "q_out"},
+                                     slot_array, position_array}))
+        return rc;
+    return launch_rotate(call, p, grid, who);
   });
 }
 

@@ -231,6 +231,25 @@ def test_index_arrays_inside_what_is_written_are_refused():
         assert _apply(r, positions=at) == ERR_INVALID and b"out shares bytes with positions" in said()
 
 
+@pytest.mark.skipif(kvt_amd.device_count() > 0, reason="this check is for machines without a GPU")
+def test_more_rows_than_a_launch_can_have_are_refused_as_such():
+    """A grid has fewer than 2^32 lanes: 16777215 workgroups of 256."""
+    said, lanes = (lambda: kvt_amd.lib().kvt_last_error()), 16777215 * 256
+    r, far = kvt_amd.Rotary(64), dict(out=P, positions=1 << 50)
+    most = lanes // (8 * 4)                                  # 8 heads of four times two 16-byte pieces
+    assert _apply(r, n=most, **far) == ctypes_defs.ERR_NO_DEVICE
+    assert _apply(r, n=most + 1, **far) == ERR_INVALID and b"too many rows" in said()
+    most = lanes // (8 * 32)                                 # unaligned: of 32 pairs
+    assert _apply(r, n=most, x=P + 2, **dict(far, out=P + 2)) == ctypes_defs.ERR_NO_DEVICE
+    assert _apply(r, n=most + 1, x=P + 2, **dict(far, out=P + 2)) == ERR_INVALID and b"too many rows" in said()
+    lay, r = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128), kvt_amd.Rotary(128)
+    fused = dict(q=P, q_tok=12288, q_out=P, qo_tok=12288, k=P + 8192, k_tok=12288, v=P + 10240, v_tok=12288,
+                 positions=1 << 50, slots=1 << 51)
+    most = lanes // ((32 + 8 + 8) * 8)
+    assert _append(lay, r, n=most, **fused) == ERR_INVALID and b"null cache" in said()
+    assert _append(lay, r, n=most + 1, **fused) == ERR_INVALID and b"too many rows" in said()
+
+
 def test_append_takes_queries_rotated_in_place_in_a_projection_that_is_fused_head_by_head():
     lay, r = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128), kvt_amd.Rotary(128)
     w = dict(q=P, q_tok=6144, q_head=768, q_heads=8, q_out=P, qo_tok=6144, qo_head=768, k=P + 256, k_tok=6144, k_head=768,
