@@ -255,7 +255,8 @@ int kvt_rotary_create(uint32_t rotary_dim, int interleaved, const double* freq, 
     if (!freq || !out) return fail(KVT_ERR_INVALID, "kvt_rotary_create: null argument");
     if (rotary_dim < 2 || rotary_dim > 256 || rotary_dim % 2 != 0)
       return fail(KVT_ERR_INVALID, "kvt_rotary_create: rotary_dim must be even, 2 to 256");
-    if (!std::isfinite(magnitude)) return fail(KVT_ERR_INVALID, "kvt_rotary_create: magnitude is not finite");
+    if (!std::isfinite(static_cast<float>(magnitude)))
+      return fail(KVT_ERR_INVALID, "kvt_rotary_create: magnitude is not finite in 32 bits");
     for (uint32_t i = 0; i < rotary_dim / 2; ++i)
       if (!std::isfinite(freq[i])) return fail(KVT_ERR_INVALID, "kvt_rotary_create: a frequency is not finite");
     std::unique_ptr<kvt_rotary> r(new kvt_rotary());

@@ -101,6 +101,11 @@ def test_rotations_out_of_range_are_refused():
     lib.kvt_rotary_destroy(None)
 
 
+@pytest.mark.parametrize("magnitude", [3.5e38, -1e39, 1e300])
+def test_a_magnitude_beyond_32_bits_is_refused(magnitude):
+    _refused(ERR_INVALID, kvt_amd.Rotary, 64, frequencies=[1.0] * 32, magnitude=magnitude)
+
+
 # The calls below are refused on the host: the pointers are never followed.
 P, POS = 1 << 20, 1 << 30
 
