@@ -970,7 +970,8 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
  * caches of its layout on its device.
  *   dtype           of q and out: BF16 or F16; the cache holds the same or E4M3
  *   softmax_scale   0 = 1 / sqrt(head_dim)
- *   logit_cap       0 = none;  window: 0 = none
+ *   logit_cap       0 = none;  window: 0 = none   (softmax_scale k_scale, logit_cap and the ratio of both are
+ *                   held in 32 bits and have to be finite there)
  *   max_seqs        most sequences of one call, up to 65535
  *   n_workspaces    how many streams and captured graphs the operator serves during its life: each
  *                   stream that launches it eagerly and each stream capture (per stream in it) takes

@@ -858,6 +858,11 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
 // keep a head's rows together 169.8 / 171.2.
 constexpr uint32_t kAbreastUnits = 8;
 
+// Whether 32 bits hold what scores are multiplied with.
+bool scores_held(float scale, float cap) {
+  return std::isfinite(scale * kLog2e) && (cap == 0 || (std::isfinite(cap * kLog2e) && std::isfinite(scale / cap)));
+}
+
 struct Launch {
   dim3 grid;
   uint32_t lds;
@@ -978,6 +983,10 @@ int kvt_decode_create(int device, const kvt_kv_layout* layout, uint32_t dtype, u
       return fail(KVT_ERR_INVALID, "kvt_decode_create: the query heads must be a multiple of the KV heads, at most 65536");
     if (!std::isfinite(softmax_scale) || !std::isfinite(logit_cap) || logit_cap < 0)
       return fail(KVT_ERR_INVALID, "kvt_decode_create: bad softmax_scale or logit_cap");
+    d->scale = softmax_scale != 0 ? softmax_scale : 1.0f / std::sqrt(static_cast<float>(layout->head_dim));
+    d->cap = logit_cap;
+    if (!scores_held(d->scale, d->cap))
+      return fail(KVT_ERR_INVALID, "kvt_decode_create: 32 bits do not hold softmax_scale or logit_cap, or their ratio");
     if (max_seqs == 0 || max_seqs > 65535 || n_workspaces == 0 || n_workspaces > 1024)
       return fail(KVT_ERR_INVALID, "kvt_decode_create: max_seqs must be in [1, 65535], n_workspaces in [1, 1024]");
     if (int rc = check_device(device)) return rc;
@@ -992,8 +1001,6 @@ int kvt_decode_create(int device, const kvt_kv_layout* layout, uint32_t dtype, u
     d->slot_heads = std::min(d->group, 16 * d->spread);
     d->window = window;
     d->max_seqs = max_seqs;
-    d->scale = softmax_scale != 0 ? softmax_scale : 1.0f / std::sqrt(static_cast<float>(layout->head_dim));
-    d->cap = logit_cap;
     d->rows = layout->n_kv_heads * d->head_rows;
     d->teams = std::max(1u, device_cu_count(device) * per_cu(layout->head_dim) / d->rows);
     d->n_wgs = d->teams * d->rows;
@@ -1060,6 +1067,9 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     if (!std::isfinite(k_scale) || !std::isfinite(v_scale) || !(k_scale > 0) || !(v_scale > 0) ||
         (!e4m3 && (k_scale != 1.0f || v_scale != 1.0f)))
       return fail(KVT_ERR_INVALID, "kvt_decode_attention: scales must be positive, and 1 for a 16-bit cache");
+    const float scale = d->scale * k_scale;
+    if (!scores_held(scale, d->cap))
+      return fail(KVT_ERR_INVALID, "kvt_decode_attention: 32 bits do not hold softmax_scale k_scale, or its ratio to logit_cap");
     const uint32_t dim = d->layout.head_dim;
     const Rows qr{q, q_token_stride, q_head_stride}, outr{out, out_token_stride, out_head_stride};
     uint64_t q_span = 0, out_span = 0;
@@ -1105,7 +1115,6 @@ int kvt_decode_attention(kvt_decode* d, const kvt_cache* cache, uint32_t layer, 
     p.visible_max = static_cast<uint32_t>(std::min<uint64_t>(static_cast<uint64_t>(table_blocks) * d->layout.ntpb, 0x7FFFFFFFull));
     p.ntpb = d->layout.ntpb, p.n_blocks = static_cast<uint32_t>(d->layout.n_blocks);
     p.n_heads = d->n_heads, p.group = d->group, p.spread = d->spread, p.head_rows = d->head_rows, p.slot_heads = d->slot_heads, p.head_dim = dim, p.window = d->window;
-    const float scale = d->scale * k_scale;
     p.scale_log2 = scale * kLog2e;
     p.cap = d->cap * kLog2e, p.cap_in = d->cap != 0 ? scale / d->cap : 0;
     p.v_scale = v_scale;

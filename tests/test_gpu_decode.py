@@ -650,6 +650,20 @@ def test_tables_and_lengths_inside_what_is_written_are_refused():
     c.check(op, c.exact())
 
 
+def test_scales_of_the_cache_whose_products_leave_32_bits_are_refused():
+    c = Case("bf16", "e4m3", "flash", [100, 64], 4, 2, 64, 16, seed=32)
+    out, _ = c.buffers()
+    for kw, k_scale in ((dict(softmax_scale=1e10), 1e30), (dict(softmax_scale=1.0, logit_cap=1e-20), 1e20)):
+        op = c.operator(**kw)
+        with pytest.raises(kvt_amd.KvtError) as e:
+            op.run(c.handle, 0, c.q, c.d_tables, c.d_lens, out, k_scale=k_scale)
+        assert e.value.code == ERR_INVALID and "32 bits" in str(e.value)
+    # large ones that do not
+    c.check(c.operator(softmax_scale=1e-20), c.exact(scale=1e-20, k_scale=1e20), k_scale=1e20)
+    c.check(c.operator(logit_cap=1e30), c.exact(cap=0.0))
+    c.check(c.operator(logit_cap=1e-20, softmax_scale=1e10), c.exact(scale=1e10, cap=1e-20))
+
+
 def test_refusals():
     c = Case("bf16", "bf16", "flash", [100, 64], 4, 2, 64, 16, seed=18)
     out, lse = c.buffers()

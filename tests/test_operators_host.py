@@ -296,6 +296,13 @@ def test_decode_create_refuses_on_the_host():
     lib.kvt_decode_destroy(None)
 
 
+@pytest.mark.parametrize("kw", [dict(logit_cap=3e38), dict(softmax_scale=3e38), dict(softmax_scale=-3e38),
+                                dict(softmax_scale=1.0, logit_cap=1e-39), dict(softmax_scale=1e30, logit_cap=1e-20)])
+def test_scales_and_caps_whose_products_leave_32_bits_are_refused(kw):
+    lay = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128)
+    _refused(ERR_INVALID, kvt_amd.DecodeAttention, 0, lay, "bf16", 32, 4, **kw)
+
+
 @pytest.mark.skipif(kvt_amd.device_count() > 0, reason="this check is for machines without a GPU")
 def test_decode_create_needs_a_device():
     lay = kvt_amd.KvLayout(ctypes_defs.SHAPE_FLASH, "bf16", 64, 16, 8, 128)
