@@ -396,6 +396,59 @@ def test_many_heads_split_so_far_that_parts_are_joined_in_two_steps(kind, cache_
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
 
 
+def _cut(lens, teams):
+    """Of every sequence that is split: (first share, whether that held something before it, number of shares)."""
+    units = [-(-n // 128) for n in lens]
+    total, before, rows = sum(units), 0, []
+    teams = min(teams, total)
+    for n in units:
+        if n:
+            w0, w1 = ((before + 1) * teams - 1) // total, ((before + n) * teams - 1) // total
+            if w1 > w0:
+                rows.append((w0, w0 * total // teams < before, w1 - w0 + 1))
+        before += n
+    return rows
+
+
+@pytest.mark.parametrize("kind,cache_kind,layout,lens,heads,kv_heads,dim,block,shares", [
+    ("bf16", "bf16", "flash", [700, 50011, 0, 3000, 41005, 5, 200], 64, 1, 128, 16, 512),
+    ("bf16", "e4m3", "hnd", [700, 85027, 33, 9000], 64, 1, 128, 32, 512),
+    ("f16", "e4m3", "flash", [700, 155057, 77], 40, 1, 64, 64, 1024),
+    ("f16", "f16", "pages", [1300, 150001, 1, 20000], 48, 1, 64, 16, 1024),
+    ("bf16", "e4m3", "ragged", [2000, 30007], 64, 2, 256, 16, 128),
+    ("f16", "f16", "flash", [1000, 33001, 129, 3000], 33, 1, 256, 48, 256)])
+def test_joins_in_two_steps_that_begin_inside_another_sequences_share(kind, cache_kind, layout, lens, heads, kv_heads, dim,
+                                                                     block, shares):
+    cut = _cut(lens, shares)
+    assert any(w0 > 0 and behind and parts > 8 for w0, behind, parts in cut), cut
+    c = Case(kind, cache_kind, layout, lens, heads, kv_heads, dim, block, seed=33)
+    op, exact = c.operator(), c.exact()
+    first = c.check(op, exact)
+    c.check(op, exact, max_len=1)                            # (unsplit: the join in one step or none)
+    for _ in range(3):
+        again = c.check(op, exact)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("kind,cache_kind,heads,kv_heads,dim,shares", [
+    ("bf16", "bf16", 64, 4, 128, 256), ("f16", "e4m3", 48, 4, 64, 512), ("bf16", "e4m3", 64, 4, 256, 128),
+    ("bf16", "bf16", 96, 6, 128, 170)])
+def test_two_heads_side_by_side_joined_in_two_steps(kind, cache_kind, heads, kv_heads, dim, shares):
+    """A table with room for far longer sequences makes the launch one for a large batch."""
+    lens = [830, 70001, 0, 5000]
+    cut = _cut(lens, shares)
+    assert any(w0 > 0 and behind and parts > 8 for w0, behind, parts in cut), cut
+    c = Case(kind, cache_kind, "flash", lens, heads, kv_heads, dim, 16, seed=34)
+    c.tables = np.pad(c.tables, ((0, 0), (0, 20000)), constant_values=-1)
+    c.d_tables = torch.from_numpy(c.tables).cuda()
+    op, exact = c.operator(), c.exact()
+    first = c.check(op, exact)
+    c.check(op, exact, max_len=70001)
+    for _ in range(3):
+        again = c.check(op, exact)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 @pytest.mark.parametrize("n", [63, 64, 65, 700])
 def test_many_short_sequences(n):
     rng = np.random.default_rng(12)
@@ -553,6 +606,28 @@ def test_streams_have_workspaces_of_their_own():
     op.release(streams[0].cuda_stream)
     op.run(a.handle, 0, a.q, a.d_tables, a.d_lens, out, lse=lse)
     hold(out, lse, exact[0], "bf16")
+
+
+def test_one_operator_from_several_threads():
+    """Calls of four threads at once, each on a stream of its own, in the order the interpreter gives them."""
+    c = Case("bf16", "bf16", "flash", [3000, 20, 700], 8, 2, 64, 16, seed=35)
+    op, exact = c.operator(workspaces=4), c.exact()
+    streams = [checkers.side_stream() for _ in range(4)]
+    buffers = [[c.buffers() for _ in range(25)] for _ in streams]
+    torch.cuda.synchronize()
+
+    def work(n):
+        for out, lse in buffers[n]:
+            op.run(c.handle, 0, c.q, c.d_tables, c.d_lens, out, lse=lse, stream=streams[n].cuda_stream)
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        list(pool.map(work, range(4)))
+    torch.cuda.synchronize()
+    one = buffers[0][0]
+    hold(*one, exact, "bf16")
+    for mine in buffers:
+        for out, lse in mine:
+            assert torch.equal(out, one[0]) and torch.equal(lse, one[1])
 
 
 def test_releasing_the_per_thread_stream_gives_back_this_threads_workspace_alone():
