@@ -961,7 +961,8 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
  * an lse of minus infinity. Rows of the cache that are not seen may hold anything, NaN included. What is
  * infinite or NaN in V of a token that is seen makes that element of the output so, however small its weight.
  * Scores, weights, sums and the maximum are held in 32 bits, the weights take part in the product
- * with V as two 16-bit values each; every output is rounded once. The same call gives the same
+ * with V as two 16-bit values each; every output is rounded once. (Sums that are divided last: values of V
+ * whose sum over the tokens leaves 32 bits give infinities.) The same call gives the same
  * bits each time; the other sequences of a batch and max_len move a sequence's result within the
  * rounding of its 32-bit sums, since they decide where it is split.
  *
@@ -979,7 +980,7 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
  *                   one; a call that finds none left is refused (KVT_ERR_INVALID). A graph must not
  *                   run at the same time as a second instantiation of itself.
  * Calls may come from several threads. Created and destroyed outside of stream captures; destroying
- * it waits for the device. */
+ * it waits for the device, and ends the use of graphs that hold its launches. */
 typedef struct kvt_decode kvt_decode;
 int kvt_decode_create(int device, const kvt_kv_layout* layout, uint32_t dtype, uint32_t n_q_heads,
                       float softmax_scale, float logit_cap, uint32_t window, uint32_t max_seqs,

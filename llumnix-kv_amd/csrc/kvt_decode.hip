@@ -26,10 +26,12 @@
 //
 // An 8-bit cache is widened on load: every e4m3 value is a bf16 and an f16 value.
 //
-// Bound by HBM once a launch has some ten microseconds of rows to read: 4 operations per cached
-// element and query head, 16 to 64 a byte, against the 180 a byte at which the matrix units would take
-// over. What the rest of this file is about is keeping enough reads in flight from every CU, and
-// leaving nothing but reads between the first row and the last:
+// Bound by HBM once a launch has some ten microseconds of rows to read. The formula has 2 operations
+// per cached element and query head; the products do 2 per element of K and 4 per element of V for 16
+// heads at a time, whether there are as many or not: 24 a byte of a 16-bit cache, 48 of an 8-bit one, for
+// every 16 query heads that share a KV head, against the 178 a byte at which the matrix units would take
+// over (more than 112 heads, or 48). What the rest of this file is about is keeping enough reads in
+// flight from every CU, and leaving nothing but reads between the first row and the last:
 //   shares   the units of 128 tokens of all sequences, one list, cut into as many equal shares as
 //            workgroups are resident, wherever that falls: no workgroup waits for a longer one, no second
 //            wave of workgroups starts (one and a half to four times as many: 131071 tokens 94 -> 100-120
@@ -48,7 +50,7 @@
 // Microseconds, and TB/s of the bytes a launch cannot do without, where a 1 GiB copy reaches 6.6: 64
 // sequences of 1k-8k tokens, 32 heads on 8 of 128 bf16, 182 (6.4); 128 of 4096, 16 on 2 of 256 f16, 160 (6.7);
 // one of 131071, 64 on 8 of 128 bf16 HND, 93 (5.8: 4 us to the first rows, 10 for the join of 64 parts);
-// 96 of 1-16384, 16 on 2 of 128 e4m3, 75 (5.2: the same, and the vector units 40 % busy with widening); one of 512, 9.1
+// 96 of 1-16384, 16 on 2 of 128 e4m3, 75 (5.2: the same, and the vector units 40 % busy with widening); one of 512, 9.0
 // (one round trip after another: lengths 1, table 2, rows 1.3, the wavefronts' join 0.4, parts out 1.3, the
 // count 0.4, parts in 2).
 #include <hip/hip_runtime.h>
@@ -223,8 +225,9 @@ __device__ __forceinline__ uint32_t units_of(const DecodeParams& p, int32_t raw)
 
 // A row's parts are joined in two steps where they are more than kFan and, together, more than kAlone float4s: one
 // workgroup reads some 25 GB/s of them. One / two steps, microseconds: 2 sequences of 65000, 64 heads on one of
-// 128, 212 / 67; one of 131071, 128 on 8 of 128 (64 parts of 512) 127 / 107; 4 of 9343, 32 on 2 of 192 (33 of 768)
-// 31.1 / 30.0 (not kept for such heads); but 64 parts of 256 92.4 / 93.5, 16 of 384 15.4 / 16.1. The code of it slows launches
+// 128, 212 / 68 (their rows take 10 at the rate of a copy: it is the join that bounds such launches); one of 131071,
+// 128 on 8 of 128 (64 parts of 512) 127 / 108; 4 of 9343, 32 on 2 of 192 (33 of 768) 31.1 / 30.0 (not kept for such
+// heads; rows 9); but 64 parts of 256 92.4 / 93.5, 16 of 384 15.4 / 16.1. The code of it slows launches
 // that do not need it (e4m3 74.2 / 75.6, 512 tokens 9.1 / 9.8), so that it is a kernel of its own, taken where
 // equally long sequences would be split that far; each of the two is right for any lengths.
 constexpr uint32_t kFan = 8, kAlone = 20480;
@@ -252,7 +255,7 @@ __device__ __forceinline__ params_t arguments() {
 
 enum { kWhole, kNear, kFar };
 
-// Workgroups of a launch, per CU: what is resident at once. Rows of 128 need 168 registers, and three
+// Workgroups of a launch, per CU: what is resident at once. Rows of 128 need 160 registers, and three
 // workgroups a CU would fit, but read no faster than two (e4m3 76.6 us against 73.9: shorter shares,
 // more parts); two of rows of 256 take 170 us where one takes 160.
 constexpr uint32_t per_cu(uint32_t dim) { return dim <= 64 ? 4 : dim <= 128 ? 2 : 1; }
