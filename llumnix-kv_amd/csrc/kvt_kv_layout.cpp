@@ -122,13 +122,13 @@ int check_apart(const Rows& in, uint32_t in_heads, const Rows& out, uint32_t out
   if (same_tokens && same_heads) {
     // rows interleave head by head (or token by token within a head): those of two tokens dt apart and two
     // heads dh apart meet where |a - b + dt token_stride + dh head_stride| < row_bytes
-    typedef __int128 wide;
-    const wide t_stride = n_tokens == 1 ? 0 : in.token_stride, most = n_tokens - 1, row = row_bytes;
-    const wide h_stride = in_heads > 1 ? in.head_stride : out_heads > 1 ? out.head_stride : 0;
-    const auto floored = [](wide n, wide d) { return n / d - (n % d < 0); };
+    // (spans stay within 62 bits and addresses far below that, so that 64 bits hold every sum)
+    const int64_t t_stride = n_tokens == 1 ? 0 : in.token_stride, most = n_tokens - 1, row = row_bytes;
+    const int64_t h_stride = in_heads > 1 ? in.head_stride : out_heads > 1 ? out.head_stride : 0;
+    const auto floored = [](int64_t n, int64_t d) { return n / d - (n % d < 0); };
     bool meet = false;
-    for (wide dh = -(static_cast<wide>(out_heads) - 1); dh < in_heads && !meet; ++dh) {
-      const wide c = static_cast<wide>(a) - static_cast<wide>(b) + dh * h_stride;
+    for (int64_t dh = -(static_cast<int64_t>(out_heads) - 1); dh < in_heads && !meet; ++dh) {
+      const int64_t c = static_cast<int64_t>(a - b) + dh * h_stride;
       if (t_stride == 0)
         meet = -row < c && c < row;
       else
