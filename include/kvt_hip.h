@@ -961,8 +961,7 @@ int kvt_kv_append(const kvt_cache* cache, uint32_t layer, const kvt_kv_layout* l
  * an lse of minus infinity. Rows of the cache that are not seen may hold anything, NaN included. What is
  * infinite or NaN in V of a token that is seen makes that element of the output so, however small its weight.
  * Scores, weights, sums and the maximum are held in 32 bits, the weights take part in the product
- * with V as two 16-bit values each; every output is rounded once. (Sums that are divided last: values of V
- * whose sum over the tokens leaves 32 bits give infinities.) The same call gives the same
+ * with V as two 16-bit values each; every output is rounded once. The same call gives the same
  * bits each time; the other sequences of a batch and max_len move a sequence's result within the
  * rounding of its 32-bit sums, since they decide where it is split.
  *

@@ -22,7 +22,8 @@
 // makes its smallest positive number 2^-40 of the largest weight: 2^-24 of it, for each of the many
 // small weights of a long sequence in which one token stands out, would add up to more than the
 // output's own rounding. (The largest weights, cut off to f16's largest number of 65504, leave the rest
-// of 65536 as any other.)
+// of 65536 as any other.) For bf16 rows they are taken times the power of two next below 1 / length,
+// so that no sum over the tokens leaves 32 bits, whatever V holds.
 //
 // An 8-bit cache is widened on load: every e4m3 value is a bf16 and an f16 value.
 //
@@ -111,7 +112,11 @@ struct Bf16 {
   static __device__ __forceinline__ uint32_t cut(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
   }
-  static constexpr float kLeast = 0x1p-126f, kTop = 1.0f;
+  template <bool E4M3>
+  static __device__ __forceinline__ float top(uint32_t len) {
+    return E4M3 ? 1.0f : __uint_as_float((95u + __builtin_clz(len)) << 23);
+  }
+  static constexpr float kLeast = 0x1p-126f;
   static constexpr uint32_t kLeastTwice = 0x00800080u;
 };
 struct F16 {
@@ -127,7 +132,9 @@ struct F16 {
   static __device__ __forceinline__ uint32_t cut(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
   }
-  static constexpr float kLeast = 0x1p-24f, kTop = 0x1p16f;
+  template <bool E4M3>
+  static __device__ __forceinline__ float top(uint32_t) { return 0x1p16f; }
+  static constexpr float kLeast = 0x1p-24f;
   static constexpr uint32_t kLeastTwice = 0x00010001u;
 };
 
@@ -384,6 +391,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
       len = seen_of(p, constant(p.lens)[++seq]);
       continue;
     }
+    const float top_weight = T::template top<E4M3>(len);
     const uint32_t unit0 = static_cast<uint32_t>(u - before);
     const uint32_t n_units = u_end - u < units - unit0 ? static_cast<uint32_t>(u_end - u) : units - unit0;
     const uint32_t begin = first + unit0 * kStep;
@@ -579,7 +587,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
         const int s = i >> 1, r = 2 * (i & 1);
         float a = __builtin_amdgcn_exp2f(sc[s][r] - ref), b = __builtin_amdgcn_exp2f(sc[s][r + 1] - ref);
         sum += a + b;
-        a *= T::kTop, b *= T::kTop;
+        a *= top_weight, b *= top_weight;
         // (positive numbers, and NaN above them, are in the order of their bits)
         const uint32_t hi = __builtin_bit_cast(
             uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, T::cut(a, b)), __builtin_bit_cast(u16x2, T::kLeastTwice)));
@@ -664,7 +672,7 @@ __global__ __launch_bounds__(kThreads, per_cu(D)) void decode_kernel(const Decod
     const uint32_t quads = dim / 4, work = heads * quads;
     const bool whole = n_units == units;
     const auto finish = [&](uint32_t head, uint32_t d, f32x4 o, float m, float l, bool nothing_but_inf) {
-      const float inv = l == 0.0f ? (nothing_but_inf ? NAN : 0.0f) : p.v_scale / T::kTop / l;
+      const float inv = l == 0.0f ? (nothing_but_inf ? NAN : 0.0f) : p.v_scale / top_weight / l;
       uint8_t* a = p.out + seq * p.out_token + (head0 + head) * p.out_head + d * 2u;
       o *= inv;
       const f32x2 lo = {o.x, o.y}, hi = {o.z, o.w};

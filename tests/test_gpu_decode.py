@@ -311,6 +311,31 @@ def test_infinities_in_v_come_through_the_join_in_two_steps(at):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("heads", [4, 64])
+@pytest.mark.parametrize("size", ["largest", "smallest"])
+def test_means_of_the_types_largest_and_smallest_values(kind, heads, size):
+    """Weights that are all alike and some that are not: sums over the tokens that are far beyond what is summed, and
+    products with small weights that are normal numbers of 32 bits by a little."""
+    lens = [700, 2, 20011, 1]
+    c = Case(kind, kind, "flash", lens, heads, 1, 64, 16, seed=36, spread=0.5)
+    info = torch.finfo(oc.torch_type(kind))
+    most = float(info.max) if size == "largest" else float(info.tiny) * (2.0 ** 17 if kind == "bf16" else 1.0)
+    c.q[0] = 0                                               # all weights alike
+    v, plain = oc.kv_views("flash", c.cache)[1].view(c.cache_type), c.plain[1]
+    for b, n in enumerate(lens):
+        t = np.arange(n)
+        page = c.tables[b][t // 16].astype(np.int64)
+        rows = torch.full((n, 1, 64), most, dtype=c.cache_type, device="cuda")
+        rows[:, :, 32:] *= -1
+        rows[1::2, :, 16:48] *= 0.5
+        v[torch.from_numpy(page).cuda(), torch.from_numpy(t % 16).cuda()] = rows
+        plain[page, t % 16] = oc.wide(rows)
+    op, exact = c.operator(), c.exact()
+    for max_len in (0, 1):
+        c.check(op, exact, max_len=max_len)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_every_8_bit_value_is_itself(kind):
     """One token: the output is its row of V, times the scale; NaN included. As keys: scores that are
     the value times a query of one."""
