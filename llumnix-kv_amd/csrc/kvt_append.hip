@@ -16,7 +16,7 @@
 // Bound by HBM: 3 operations per element moved. Microseconds a call, and TB/s of what it reads and
 // writes, where a 1 GiB copy reaches 6.6: 16384 x 64 rows of 128 f16, interleaved, 85 (6.3); a prompt of
 // 16384, heads of 32 + 8 + 8 x 128 bf16, 67 (6.0); one of 10007, 16 + 2 + 2 x 256, to e4m3 pages, 33 (5.9).
-// A step of few tokens is one round trip to memory after a launch: 2.5 for one token, 4.0 for 256 x 80
+// A step of few tokens is one round trip to memory after a launch: 2.6 for one token, 4.0 for 256 x 80
 // rows of 128, less than a caller's host needs to issue it.
 #include <hip/hip_runtime.h>
 

@@ -108,7 +108,7 @@ struct Bf16 {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(e4m3, 1.0f, HIGH));
   }
   // two values cut off to this type, its smallest positive number (here of the normal ones) and
-  // the bits of two of them, and what the largest weight is in the product with V
+  // the bits of two of them, and what the largest weight of a sequence is in the product with V
   static __device__ __forceinline__ uint32_t cut(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
   }
